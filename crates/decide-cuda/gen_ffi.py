@@ -15,7 +15,8 @@ HEADER = ROOT / "include" / "decide_cuda.h"
 OUT = Path(__file__).resolve().parent / "src" / "ffi.rs"
 
 SCALARS = {"int": "i32", "uint32_t": "u32", "uint64_t": "u64", "size_t": "usize", "float": "f32", "char": "c_char", "void": "c_void",
-           "dc_ctx": "DcCtx", "dc_model": "DcModel", "dc_dims": "DcDims", "dc_layer_weights": "DcLayerWeights", "dc_convert_report": "DcConvertReport"}
+           "dc_ctx": "DcCtx", "dc_model": "DcModel", "dc_dims": "DcDims", "dc_layer_weights": "DcLayerWeights", "dc_convert_report": "DcConvertReport",
+           "dc_kv8_cache": "DcKv8Cache"}
 KEYWORDS = {"type", "ref", "in", "impl", "mod", "move", "fn", "match", "loop", "where"}
 
 
@@ -63,8 +64,16 @@ def render() -> str:
              "pub struct DcLayerWeights {", "    pub in_norm: *const f32, pub w_in: *const c_void, pub w_out: *const c_void, pub post_norm: *const f32,",
              "    pub w_gu: *const c_void, pub w_down: *const c_void, pub conv_w: *const f32, pub a_log: *const f32, pub dt_bias: *const f32,",
              "    pub gnorm: *const f32, pub q_norm: *const f32, pub k_norm: *const f32,", "}", "",
+             "/// dc_kv8_cache: a paged 8-bit K/V cache: device pointers, strides in codes, dims.",
+             "#[repr(C)] #[derive(Clone, Copy, Debug)]",
+             "pub struct DcKv8Cache {", "    pub k: *mut c_void, pub v: *mut c_void, pub k_scale: *mut f32, pub v_scale: *mut f32,",
+             "    pub table: *mut u32, pub lens: *mut u32, pub refs: *mut u32,",
+             "    pub layer_stride: u64, pub page_stride: u64, pub head_stride: u64, pub token_stride: u64,",
+             "    pub layers: u32, pub n_pages: u32, pub nkv: u32, pub page_size: u32, pub hd: u32, pub n_seqs: u32, pub max_pages: u32,",
+             "    pub reserved: u32,", "}", "",
              "pub const DC_OK: i32 = 0;", "pub const DC_INVALID_ARG: i32 = 1;", "pub const DC_CUDA_ERROR: i32 = 2;", "pub const DC_UNSUPPORTED: i32 = 3;",
-             "pub const DC_TIMEOUT: i32 = 4;", "pub const DC_NOALLOC_MAX_VALUES: u64 = 1 << 32;", "pub const DC_GEMM_SMALL_MAX_M: u32 = 16;", "",
+             "pub const DC_TIMEOUT: i32 = 4;", "pub const DC_NOALLOC_MAX_VALUES: u64 = 1 << 32;", "pub const DC_GEMM_SMALL_MAX_M: u32 = 16;",
+             "pub const DC_KV8_NO_KEYS: u32 = 0xFFFF_FFFF;", "",
              '#[link(name = "decide_cuda")]', 'extern "C" {']
     for name, args, ret in prototypes(HEADER.read_text()):
         sig = ", ".join(f"{a}: {t}" for a, t in args)

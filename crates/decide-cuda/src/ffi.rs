@@ -26,6 +26,16 @@ pub struct DcLayerWeights {
     pub gnorm: *const f32, pub q_norm: *const f32, pub k_norm: *const f32,
 }
 
+/// dc_kv8_cache: a paged 8-bit K/V cache: device pointers, strides in codes, dims.
+#[repr(C)] #[derive(Clone, Copy, Debug)]
+pub struct DcKv8Cache {
+    pub k: *mut c_void, pub v: *mut c_void, pub k_scale: *mut f32, pub v_scale: *mut f32,
+    pub table: *mut u32, pub lens: *mut u32, pub refs: *mut u32,
+    pub layer_stride: u64, pub page_stride: u64, pub head_stride: u64, pub token_stride: u64,
+    pub layers: u32, pub n_pages: u32, pub nkv: u32, pub page_size: u32, pub hd: u32, pub n_seqs: u32, pub max_pages: u32,
+    pub reserved: u32,
+}
+
 pub const DC_OK: i32 = 0;
 pub const DC_INVALID_ARG: i32 = 1;
 pub const DC_CUDA_ERROR: i32 = 2;
@@ -33,6 +43,7 @@ pub const DC_UNSUPPORTED: i32 = 3;
 pub const DC_TIMEOUT: i32 = 4;
 pub const DC_NOALLOC_MAX_VALUES: u64 = 1 << 32;
 pub const DC_GEMM_SMALL_MAX_M: u32 = 16;
+pub const DC_KV8_NO_KEYS: u32 = 0xFFFF_FFFF;
 
 #[link(name = "decide_cuda")]
 extern "C" {
@@ -92,6 +103,15 @@ extern "C" {
     pub fn dc_attention_scratch_bytes(rows: u32, n_seq: u32, nkv: u32) -> usize;
     pub fn dc_conv_gated_delta(ctx: *mut DcCtx, stream: *mut c_void, p: *const f32, prev: *const f32, w: *const f32, a: *const f32, b: *const f32, a_log: *const f32, dt_bias: *const f32, state_in: *const f32, state_out: *mut f32, o: *mut f32, t: u32, ldp: u32, write_state: u32, nk: u32, nv: u32, dk: u32, dv: u32, seq_start: *const u32, n_seq: u32, max_len: u32) -> i32;
     pub fn dc_conv_gated_delta_supported(ctx: *mut DcCtx) -> i32;
+    pub fn dc_kv8_check(cache: *const DcKv8Cache, err: *mut c_char, err_len: usize) -> i32;
+    pub fn dc_kv8_extend(ctx: *mut DcCtx, stream: *mut c_void, cache: *const DcKv8Cache, add: *const u32) -> i32;
+    pub fn dc_kv8_fork(ctx: *mut DcCtx, stream: *mut c_void, cache: *const DcKv8Cache, src: *const u32, dst: *const u32, n: u32, deep: u32) -> i32;
+    pub fn dc_kv8_free(ctx: *mut DcCtx, stream: *mut c_void, cache: *const DcKv8Cache, seqs: *const u32, n: u32) -> i32;
+    pub fn dc_kv8_compact(ctx: *mut DcCtx, stream: *mut c_void, cache: *const DcKv8Cache, live: *mut u32) -> i32;
+    pub fn dc_kv8_pages_scratch_bytes(cache: *const DcKv8Cache) -> usize;
+    pub fn dc_kv8_append(ctx: *mut DcCtx, stream: *mut c_void, cache: *const DcKv8Cache, layer: u32, k: *const c_void, v: *const c_void, ldk: u32, ldv: u32, row_start: *const u32, rows: u32, max_rows: u32) -> i32;
+    pub fn dc_kv8_attention(ctx: *mut DcCtx, stream: *mut c_void, cache: *const DcKv8Cache, layer: u32, q: *const c_void, gate: *const f32, q_start: *const u32, qpos: *const u32, y: *mut c_void, rows: u32, ldq: u32, ldg: u32, ldy: u32, nq: u32, max_q: u32, max_len: u32) -> i32;
+    pub fn dc_kv8_attention_scratch_bytes(ctx: *mut DcCtx, cache: *const DcKv8Cache, nq: u32, max_q: u32, max_len: u32) -> usize;
     pub fn dc_model_create(ctx: *mut DcCtx, dims: *const DcDims, layers: *const DcLayerWeights, embed: *const c_void, final_norm: *const f32, max_rows: u32, max_seqs: u32, max_answers: u32, max_cand: u32) -> *mut DcModel;
     pub fn dc_model_destroy(m: *mut DcModel);
     pub fn dc_model_activation_bytes(m: *mut DcModel) -> usize;

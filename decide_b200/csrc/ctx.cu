@@ -5,6 +5,7 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "kv8.cuh"
 
 int dc_fail(dc_ctx* ctx, int code, const char* fmt, ...) {
     char buf[512];
@@ -45,6 +46,21 @@ int dc_get_workspace(dc_ctx* ctx, size_t bytes, const char* who, void** out) {
     ctx->workspace_bytes = bytes ? bytes : 256;
     *out = p;
     return DC_OK;
+}
+
+// Messages of the violations that only the dc_kv8_* kernels can see; null for other codes.
+static const char* dc_kv8_status_text(int code) {
+    switch (code) {
+        case DC_STATUS_KV8_OFFSETS: return "kv8: row offsets fall, pass the number of rows, or give a sequence more rows than the maximum given or than it has tokens; its rows were skipped";
+        case DC_STATUS_KV8_LENGTH: return "kv8: a sequence is longer than its row of the page table can hold, or than the max_len given";
+        case DC_STATUS_KV8_PAGE: return "kv8: the page table names a page outside the pool";
+        case DC_STATUS_KV8_POSITION: return "kv8: a query row's position lies at or past the length of its sequence";
+        case DC_STATUS_KV8_SHARED: return "kv8: rows for a page that is free or that several sequences hold; they were not written";
+        case DC_STATUS_KV8_POOL: return "kv8: too few free pages; the call changed nothing";
+        case DC_STATUS_KV8_SEQUENCE: return "kv8: a sequence index is out of range or named twice";
+        case DC_STATUS_KV8_REFS: return "kv8: a page was freed more often than it was held";
+        default: return nullptr;
+    }
 }
 
 static uint32_t impl_from_env(const char* name, bool* bad) {
@@ -229,6 +245,7 @@ int dc_check_status(dc_ctx* ctx, void* stream) {
         cudaStreamSynchronize(s);
         if (code == DC_STATUS_POSITION_PAST_CACHE)
             return dc_fail(ctx, DC_INVALID_ARG, "attention: a query row's position lies at or past the cache length given as max_len; the results of this run are invalid");
+        if (const char* what = dc_kv8_status_text(code)) return dc_fail(ctx, DC_INVALID_ARG, "%s", what);
         return dc_fail(ctx, DC_TIMEOUT, "a bounded device-side wait ran out (wait id %d); the results of this run are invalid", code);
     }
     return DC_OK;
@@ -260,6 +277,7 @@ int dc_warm_up(dc_ctx* ctx) {
     if (rc == DC_OK) rc = dc_attention_warm(ctx);
     if (rc == DC_OK) rc = dc_attention_tc_warm(ctx);
     if (rc == DC_OK) rc = dc_delta_chunk_warm(ctx);
+    if (rc == DC_OK) rc = dc_kv8_attention_warm(ctx);
     return rc;
 }
 

@@ -67,6 +67,59 @@ class ConvertReport(ctypes.Structure):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}
 
 
+class _Kv8Struct(ctypes.Structure):
+    """dc_kv8_cache."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table", "lens", "refs")]
+                + [(n, ctypes.c_uint64) for n in ("layer_stride", "page_stride", "head_stride", "token_stride")]
+                + [(n, ctypes.c_uint32) for n in ("layers", "n_pages", "nkv", "page_size", "hd", "n_seqs", "max_pages", "reserved")])
+
+
+class Kv8Cache:
+    """A paged 8-bit K/V cache over the caller's tensors (dc_kv8_cache in include/decide_cuda.h has the rules):
+
+    k, v      e4m3 codes (torch.float8_e4m3fn or uint8) [layers, n_pages, nkv, page_size, hd]; any strides alike for both (a permuted view
+              of [layers, n_pages, page_size, nkv, hd] is fine), the last dim contiguous
+    k_scale, v_scale  fp32 [layers, n_pages, nkv]
+    table     int32 [n_seqs, max_pages], lens int32 [n_seqs], refs int32 [n_pages]
+
+    `Kv8Cache.empty` makes an empty one. The tensors are the cache's state: it keeps them alive and the kernels write them."""
+
+    def __init__(self, k, v, k_scale, v_scale, table, lens, refs):
+        def need(ok, what):
+            if not ok:
+                raise KernelError(1, f"Kv8Cache: {what}")
+
+        need(k.dim() == 5 and k.shape == v.shape, "k and v are [layers, n_pages, nkv, page_size, hd]")
+        need(all(t.dtype in (torch.uint8, torch.float8_e4m3fn) for t in (k, v)), "k and v hold e4m3 codes (float8_e4m3fn or uint8)")
+        need(k.stride() == v.stride() and k.stride(4) == 1, "k and v have the same strides and contiguous rows")
+        layers, n_pages, nkv, page_size, hd = k.shape
+        for name, t, shape, dtype in (("k_scale", k_scale, (layers, n_pages, nkv), torch.float32), ("v_scale", v_scale, (layers, n_pages, nkv), torch.float32),
+                                      ("table", table, tuple(table.shape), torch.int32), ("lens", lens, (table.shape[0],), torch.int32),
+                                      ("refs", refs, (n_pages,), torch.int32)):
+            need(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous(), f"{name} is a contiguous {dtype} tensor of shape {list(shape)}")
+        need(table.dim() == 2, "table is [n_seqs, max_pages]")
+        need(all(t.device == k.device for t in (v, k_scale, v_scale, table, lens, refs)), "all tensors are on one device")
+        self.k, self.v, self.k_scale, self.v_scale, self.table, self.lens, self.refs = k, v, k_scale, v_scale, table, lens, refs
+        self.layers, self.n_pages, self.nkv, self.page_size, self.hd = layers, n_pages, nkv, page_size, hd
+        self.n_seqs, self.max_pages = table.shape
+        self.struct = _Kv8Struct(*(t.data_ptr() for t in (k, v, k_scale, v_scale, table, lens, refs)), *(k.stride(i) for i in range(4)), layers, n_pages, nkv,
+                                 page_size, hd, *table.shape, 0)
+        self.ref = ctypes.addressof(self.struct)
+        err = ctypes.create_string_buffer(160)
+        rc = _lib.load().dc_kv8_check(self.ref, err, len(err))
+        if rc != 0:
+            raise KernelError(rc, f"Kv8Cache: {err.value.decode()}")
+
+    @classmethod
+    def empty(cls, layers: int, n_pages: int, nkv: int, hd: int, n_seqs: int, max_pages: int, page_size: int = 64, device="cuda"):
+        """A cache of free pages and sequences of no tokens."""
+        shape = (layers, n_pages, nkv, page_size, hd)
+        codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+        scales = [torch.full(shape[:3], 2.0 ** -60, device=device) for _ in range(2)]
+        ints = [torch.zeros(s, dtype=torch.int32, device=device) for s in ((n_seqs, max_pages), (n_seqs,), (n_pages,))]
+        return cls(*codes, *scales, *ints)
+
+
 def _ptr(arg) -> int:
     """Device address of a tensor, or of (tensor, byte offset); None -> NULL."""
     if arg is None:
@@ -362,6 +415,47 @@ class Delta(_Family):
                       _ptr(state_in), _ptr(state_out), _ptr(o), t, ldp, int(write_state), nk, nv, dk, dv, _ptr(seq_start), n_seq, max_len)
 
 
+class Kv8(_Family):
+    """The paged 8-bit K/V cache (no counterpart in the reference): include/decide_cuda.h, dc_kv8_*. Index tensors are int32 (u32 in C);
+    `stream` None is the current stream of the context's device."""
+
+    def _stream(self, stream) -> int:
+        return torch.cuda.current_stream(self.dev.device).cuda_stream if stream is None else _stream(stream)
+
+    def extend(self, stream, cache: Kv8Cache, add):
+        """Lengthens sequence j by add[j] tokens: gives it the pages it lacks."""
+        self.dev.call("dc_kv8_extend", self._stream(stream), cache.ref, _ptr(add))
+
+    def fork(self, stream, cache: Kv8Cache, src, dst, n: int, deep: bool = False):
+        """Sequence dst[i] becomes a copy of src[i]: it shares the full pages (deep: gets copies of all)."""
+        self.dev.call("dc_kv8_fork", self._stream(stream), cache.ref, _ptr(src), _ptr(dst), n, int(deep))
+
+    def free(self, stream, cache: Kv8Cache, seqs, n: int):
+        """Frees sequences seqs[0 .. n)."""
+        self.dev.call("dc_kv8_free", self._stream(stream), cache.ref, _ptr(seqs), n)
+
+    def compact(self, stream, cache: Kv8Cache, live=None):
+        """Moves the pages in use to the lowest ids; live[0] (int32, may be None) receives how many there are."""
+        self.dev.call("dc_kv8_compact", self._stream(stream), cache.ref, _ptr(live))
+
+    def append(self, stream, cache: Kv8Cache, layer: int, k, v, ldk: int, ldv: int, row_start, rows: int, max_rows: int):
+        """Writes rows row_start[j] .. row_start[j+1] of k and v as the last tokens of sequence j."""
+        self.dev.call("dc_kv8_append", self._stream(stream), cache.ref, layer, _ptr(k), _ptr(v), ldk, ldv, _ptr(row_start), rows, max_rows)
+
+    def attention(self, stream, cache: Kv8Cache, layer: int, q, gate, q_start, qpos, y, rows: int, ldq: int, ldg: int, ldy: int, nq: int, max_q: int,
+                  max_len: int = 0):
+        """Causal GQA attention of rows q_start[j] .. q_start[j+1] over sequence j, with the optional sigmoid gate; qpos None: the rows
+        are the sequence's last tokens."""
+        self.dev.call("dc_kv8_attention", self._stream(stream), cache.ref, layer, _ptr(q), _ptr(gate), _ptr(q_start), _ptr(qpos), _ptr(y), rows, ldq, ldg,
+                      ldy, nq, max_q, max_len)
+
+    def pages_scratch_bytes(self, cache: Kv8Cache) -> int:
+        return int(self.dev.lib.dc_kv8_pages_scratch_bytes(cache.ref))
+
+    def attention_scratch_bytes(self, cache: Kv8Cache, nq: int, max_q: int, max_len: int = 0) -> int:
+        return int(self.dev.lib.dc_kv8_attention_scratch_bytes(self.dev.handle, cache.ref, nq, max_q, max_len))
+
+
 class Kernels:
     """Every kernel family, as `Kernels::new(dev)` of the reference (kernels/mod.rs:54-66)."""
 
@@ -376,3 +470,4 @@ class Kernels:
         self.attn = Attn(dev)
         self.conv = Conv(dev)
         self.delta = Delta(dev)
+        self.kv8 = Kv8(dev)

@@ -358,6 +358,93 @@ int dc_conv_gated_delta(dc_ctx* ctx, void* stream, const float* p, const float* 
 int dc_conv_gated_delta_supported(dc_ctx* ctx);
 
 /* ======================================================================================
+ * Paged 8-bit K/V cache (no counterpart in the reference, whose caches are 16-bit and one per run): half the
+ * bytes per token, and states that share their pages, so that many follow-up questions hold one request's state.
+ *
+ * A page holds page_size tokens of one layer for every kv head, K and V apart, as e4m3 codes (4-bit exponent, 3-bit
+ * mantissa, largest 448), with one fp32 scale per (layer, page, kv head) for K and one for V: value = code * scale.
+ * Scales are powers of two, the least 2^e >= 2^-60 with 448 * 2^e >= the largest magnitude the page has held for
+ * that head; a scale never falls while the page is in use, and when new rows raise it the codes already there are
+ * rounded again, to nearest even. A (page, head) that has taken in a value that is not finite has the scale NaN
+ * from then on (the codes of its new rows are zero): what attends it is NaN, nothing else is.
+ * A page id means the same page in every layer. Sequence j is row j of `table` (the ids of its pages in order)
+ * and lens[j], the tokens it holds; refs[p] counts the sequences that hold page p, 0 = free. Sequences share whole
+ * pages only. All arrays are device memory of the caller; nothing but these entry points needs to write them
+ * (start from lens = 0 and refs = 0).
+ *
+ * What only the device can see (table, lens, refs, offsets, positions) is checked there: a violation raises the
+ * status word, is reported by the next dc_check_status as DC_INVALID_ARG, and never reads or writes outside the
+ * arrays described here. Unless an entry point says otherwise, what it concerns is skipped.
+ * ====================================================================================== */
+typedef struct dc_kv8_cache {
+    void* k;                      /* e4m3 codes, 16-byte aligned; k and v have the same strides, in codes, multiples of 16: */
+    void* v;                      /* code (layer, page, head, token, dim) at layer*layer_stride + page*page_stride + head*head_stride + token*token_stride + dim */
+    float* k_scale;               /* [layers][n_pages][nkv] */
+    float* v_scale;
+    uint32_t* table;              /* [n_seqs][max_pages] */
+    uint32_t* lens;               /* [n_seqs] */
+    uint32_t* refs;               /* [n_pages] */
+    uint64_t layer_stride, page_stride, head_stride, token_stride;
+    uint32_t layers, n_pages, nkv, page_size, hd, n_seqs, max_pages;
+    uint32_t reserved;            /* 0 */
+} dc_kv8_cache;
+
+/* qpos of a padding row of dc_kv8_attention: it attends nothing and its output is zero. */
+#define DC_KV8_NO_KEYS 0xFFFFFFFFu
+
+/* Checks the description alone (pointers set and aligned, page_size 16 | 32 | 64 | 128, hd 128 | 256, strides that keep
+ * codes apart, n_seqs <= 65535, n_pages <= 2^21, max_pages * page_size < 2^31): DC_OK, or DC_INVALID_ARG / DC_UNSUPPORTED with a message in
+ * `err` (may be NULL). Needs no GPU and no context. Every dc_kv8_* entry point makes the same checks. */
+int dc_kv8_check(const dc_kv8_cache* cache, char* err, size_t err_len);
+
+/* Lengthens sequence j by add[j] tokens (u32 [n_seqs]): gives it the pages it lacks, lowest free id first in the order
+ * of the sequences, and raises lens[j]. All or nothing: where the pool has too few free pages, or a sequence would
+ * outgrow its row of the table, the call changes nothing and raises the status word. The tokens' codes are written by
+ * dc_kv8_append. Scratch: dc_kv8_pages_scratch_bytes. */
+int dc_kv8_extend(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, const uint32_t* add);
+
+/* Sequence dst[i] becomes a copy of sequence src[i] (i < n; u32 [n] each): what dst[i] held is freed first. deep = 0: it
+ * shares the full pages of src[i] (refs + 1) and gets a page of its own with a copy of the last, partly filled one; deep
+ * = 1: it gets copies of all of them. New pages are the lowest free ids, in the order of i and then of the pages; all
+ * layers' codes and scales are copied. A sequence may be the source of several copies; one named twice in dst, or in dst and
+ * in src, is a violation. All or nothing, as dc_kv8_extend. */
+int dc_kv8_fork(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, const uint32_t* src, const uint32_t* dst, uint32_t n, uint32_t deep);
+
+/* Frees sequences seqs[i] (u32 [n]): refs - 1 for each of their pages, lens = 0. A free sequence is left as it is, and
+ * so is one that is named again. Rows of the table keep their contents. */
+int dc_kv8_free(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, const uint32_t* seqs, uint32_t n);
+
+/* Moves the pages in use to the lowest ids: with L pages in use, the i-th page in use at or past L goes to the i-th
+ * free page below L, in every layer, and table and refs follow. *live (u32, device, may be NULL) = L: ids from L on are free,
+ * and their memory may be given back. */
+int dc_kv8_compact(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t* live);
+size_t dc_kv8_pages_scratch_bytes(const dc_kv8_cache* cache);
+
+/* Writes new rows of one layer. Rows row_start[j] .. row_start[j+1] of k and v (the context's 16-bit type, row r's heads
+ * side by side at r * ldk, r * ldv; u32 [n_seqs+1] offsets, ascending, at most max_rows a sequence, none past `rows`) are the LAST
+ * tokens of sequence j, which dc_kv8_extend has made room for: they go to positions lens[j] - count .. lens[j] - 1. Rows at and
+ * past row_start[n_seqs] are not read. A page that is free or that several sequences hold is not written (a violation).
+ * A page whose first token is among the new ones starts a new scale. k, v 16-byte aligned, ldk, ldv >= nkv * hd and
+ * multiples of 8. Writing the same rows again leaves the same cache. */
+int dc_kv8_append(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t layer, const void* k, const void* v, uint32_t ldk,
+                  uint32_t ldv, const uint32_t* row_start, uint32_t rows, uint32_t max_rows);
+
+/* Causal GQA attention over one layer: dc_attention's contract with this cache in the place of the 16-bit one. Query rows
+ * q_start[j] .. q_start[j+1] (u32 [n_seqs+1], ascending, at most max_q a sequence, none past `rows`) of q (the context's 16-bit type,
+ * row stride ldq, heads side by side) belong to sequence j; the row at position p attends its tokens 0 ..= p; p = qpos[row]
+ * (u32 [rows]), or with qpos NULL the sequence's rows are its last tokens. A row of DC_KV8_NO_KEYS, and every row of an empty
+ * sequence, attends nothing: its output is zero. A position at or past lens[j] is a violation (the row attends all tokens there
+ * are); a page id outside the pool makes the rows that attend it NaN. scale hd^-1/2, fp32 scores and softmax; the weights of the
+ * V product are rounded to fp16 (they are at most 2^8 of the row's largest term). `gate` (fp32, row stride ldg, NULL = none)
+ * multiplies the output by sigmoid(gate). Writes rows below q_start[n_seqs] of y (the 16-bit type, row stride ldy), no others.
+ * nq / nkv <= 16; q, y, gate 16-byte aligned, ldq, ldy multiples of 8, ldg of 4, each >= nq * hd. max_len: the longest
+ * sequence, or more (it sizes the split of the keys; 0 = max_pages * page_size); a longer one is a violation. Scratch: dc_kv8_attention_scratch_bytes. */
+int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t layer, const void* q, const float* gate,
+                     const uint32_t* q_start, const uint32_t* qpos, void* y, uint32_t rows, uint32_t ldq, uint32_t ldg, uint32_t ldy,
+                     uint32_t nq, uint32_t max_q, uint32_t max_len);
+size_t dc_kv8_attention_scratch_bytes(dc_ctx* ctx, const dc_kv8_cache* cache, uint32_t nq, uint32_t max_q, uint32_t max_len);
+
+/* ======================================================================================
  * Whole-model prefill: the host loop of Forward (crates/decide-engine/src/forward.rs:1129-1328)
  * in C++ over the entry points above, for a batch of packed requests.
  * ====================================================================================== */
