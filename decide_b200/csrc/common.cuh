@@ -42,6 +42,7 @@ struct dc_ctx {
     uint32_t act_dtype = DC_ACT_F16;  // type of every 16-bit GEMM operand: activations and weight matrices
     float* gemm_part_ws = nullptr;   // partial accumulators of K-split tail tiles: sm_count x 128 x 256 fp32
     int* gemm_part_cnt = nullptr;    // arrival counters of split tiles: sm_count x 4 row quadrants, zero between launches
+    uint32_t* kv8_done = nullptr;    // arrival counters of split attention tiles (DC_KV8_DONE_COUNTERS), zero between launches
     void* workspace = nullptr;       // scratch for the chunked delta rule and other multi-pass ops
     size_t workspace_bytes = 0;
     bool workspace_frozen = false;   // an op that needs more scratch than is reserved fails instead of allocating
@@ -51,6 +52,8 @@ struct dc_ctx {
     uint32_t tp_world = 1, tp_rank = 0;
     bool tp_exchange16 = false;      // partial sums cross the links in the 16-bit type (half the bytes) instead of fp32
 };
+
+#define DC_KV8_DONE_COUNTERS 65536u
 
 int dc_fail(dc_ctx* ctx, int code, const char* fmt, ...);
 int dc_check_launch(dc_ctx* ctx, const char* what);

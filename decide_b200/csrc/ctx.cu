@@ -154,6 +154,13 @@ dc_ctx* dc_open(int device, char* err, size_t err_len) {
         return nullptr;
     }
     ctx->allocs += 2;
+    if ((e = cudaMalloc(&ctx->kv8_done, DC_KV8_DONE_COUNTERS * sizeof(uint32_t))) != cudaSuccess ||
+        (e = cudaMemset(ctx->kv8_done, 0, DC_KV8_DONE_COUNTERS * sizeof(uint32_t))) != cudaSuccess) {
+        say("dc_open: cannot allocate the attention counters", cudaGetErrorString(e));
+        dc_close(ctx);
+        return nullptr;
+    }
+    ctx->allocs++;
     return ctx;
 }
 
@@ -164,6 +171,7 @@ void dc_close(dc_ctx* ctx) {
     if (ctx->status_dev) cudaFree(ctx->status_dev);
     if (ctx->status_host) cudaFreeHost(ctx->status_host);
     if (ctx->workspace) cudaFree(ctx->workspace);
+    if (ctx->kv8_done) cudaFree(ctx->kv8_done);
     if (ctx->gemm_part_ws) cudaFree(ctx->gemm_part_ws);
     if (ctx->gemm_part_cnt) cudaFree(ctx->gemm_part_cnt);
     delete ctx;

@@ -4,19 +4,28 @@
 // s_j = a_j (q . k'_j) hd^-1/2 and o = sum_j softmax(s)_j b_j v'_j. Taking the V scale into the exponent, with t_j = s_j log2(e) + e_v(j):
 //     o = sum_j 2^(t_j - m) v'_j / sum_j 2^(t_j - m) 2^-e_v(j),    m any upper bound of t_j up to a factor,
 // so that one running maximum serves both sums, the weights of the V product are relative to the row's largest TERM, and no code is
-// ever scaled: codes go into the tensor cores as fp16, exactly. The sum of the weights is fp32, before they are rounded to fp16.
+// ever scaled: codes go into the tensor cores as fp16, exactly. The weights are rounded once, to fp16, because the V product takes
+// 16-bit operands (relative to the row's largest term they lose nothing that matters); the total adds them in fp32 before that, since
+// a key whose page has a small V scale may weigh much in it and little in the product.
 //
-// K/V bytes bound it when there are few rows. A tile of up to 16 (query row, head of the group) pairs shares a kv head's codes; the
-// warps of a CTA take 16 keys each in turn with mma.sync m16n8k16, and everything a lane needs of a key it loads itself:
-//   K: lane (g, t) = (lane / 4, lane % 4) holds key g's codes 64 i + 16 t .. + 15; the order of the products over hd is free as long as
-//      q follows it, so four consecutive codes are the lane's B fragment of one k-step.
-//   V: lane (g, t) holds codes 128 i + 16 g .. + 15 of keys 2t, 2t+1, 2t+8, 2t+9: as B fragments these are 16 output columns
-//      (column g of tile b is hd index 128 i + 16 g + b), and the C fragments end up as 32 consecutive outputs a lane.
-// So codes go from memory to fragments with 16-byte asynchronous copies into lane-private shared memory (a ring of stages a warp,
-// no barriers, no bank conflicts) and a few integer instructions: code s eeee mmm becomes fp16 s 0eeee mmm 0000000, which is
-// value * 2^-8, exactly, subnormals included; the 2^8 joins the scale of the scores and of the output.
-// Keys are cut into chunks of kChunk over CTAs when a sequence is longer than that; partial results meet in the workspace and a
-// second kernel joins them in chunk order, so that the result does not depend on timing.
+// K/V bytes bound it when there are few rows. A CTA takes up to 8 NT (query row, head of the group) pairs that share a kv head's codes; its
+// warps take 16 keys each in turn with mma.sync m16n8k16, codes as the A operand (so that 16 keys, or 16 columns of V, fill it, and
+// a tile of 8 pairs costs HD / 8 MMAs), and everything a lane needs of a key it loads itself:
+//   S^T = K Q^T: lane (g, t) = (lane / 4, lane % 4) holds codes 64 i + 16 t .. + 15 of keys g and g + 8; the order of the products over hd
+//      is free as long as q follows it, so four consecutive codes are the lane's share of one k-step.
+//   O^T = V^T P^T: lane (g, t) holds codes 128 i + 16 g .. + 15 of keys 2t, 2t+1, 2t+8, 2t+9: as A fragments these are 16 columns,
+//      two to a tile, and the C fragments end up as 16 consecutive outputs of a pair. P^T comes from the C fragments of S^T by
+//      movmatrix.
+// Codes go from memory to fragments with 16-byte asynchronous copies of whole rows into a ring of stages that belongs to the warp (no CTA
+// barriers), 16-byte reads, a byte permutation for V and one conversion for two codes. A stage holds 16 rows of K, then of V; the
+// 16-byte pieces of each 128 bytes of a row lie at piece ^ 4 (row & 1) for K and piece ^ (row & 6) for V: a row is written in
+// one pass over the banks, and the eight lanes of a read's phase, two keys by four pieces of K or four keys by two of V, meet all 32
+// banks. (Pieces lying where their lanes read them were written four passes a row: 201 instead of 68 a tile, which bound the kernel.)
+// Codes that append has written are finite; what lies behind a sequence's last token may be the code for NaN, and a weight of zero
+// would not hide it: those V codes are replaced by zeros.
+// Keys are cut into chunks over CTAs; partial results meet in the workspace, and the CTA of a tile that finishes last (a counter tells)
+// joins them in chunk order, so that the result does not depend on timing.
+#include <cmath>
 #include "kv8.cuh"
 #include "ptx.cuh"
 
@@ -24,23 +33,26 @@ namespace {
 
 using namespace dc;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
 constexpr uint32_t kTile = 16;       // keys a warp takes at a time; a page holds a whole number of tiles
-constexpr uint32_t kMaxChunk = 32 * kWarps * kTile;   // a lane remembers the page of one of its warp's tiles: 32 tiles a warp
 constexpr float kNone = -1e30f;      // running maximum of a row that has seen nothing
 constexpr float kStep = 8.0f;        // the maximum follows only when it grows by more than 2^8
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int HD>
+template <int HD, int NT>
 struct Shape {
+    static constexpr int kWarps = HD * NT <= 256 && HD == 128 ? 8 : 4;
+    static constexpr int kThreads = 32 * kWarps;
     static constexpr int kStages = 3;
-    static constexpr int kVec = 16 * HD / 16 / 32 * 2;              // 16-byte vectors a lane holds of a tile: K, then V
+    static constexpr int kPairs = 8 * NT;
+    static constexpr int kVec = HD / 16;                            // 16-byte vectors a lane holds of a tile: half K, half V
     static constexpr size_t kStage = static_cast<size_t>(kVec) * 512;   // bytes of a warp's stage
     static constexpr size_t kRing = kWarps * kStages * kStage;
-    static constexpr size_t kQ = HD / 16 * 512;                     // q fragments: [k-step][lane] 16 bytes
-    static constexpr size_t kBytes = kRing + kQ + 2 * 16 * 4;
-    static_assert(kWarps * 16 * (HD + 2) * 4 <= kRing + kQ, "the warps' partial results reuse the ring");
+    static constexpr int kLd = HD + 4;                              // floats of a pair's partial result: sums, maximum, total
+    static constexpr size_t kParts = static_cast<size_t>(kWarps) * kPairs * kLd * 4;   // the warps' results reuse the ring
+    static constexpr size_t kQ = kRing > kParts ? kRing : kParts;   // offset of the q fragments: [k-step][8 pairs][lane] 8 bytes
+    static constexpr size_t kSeen = kQ + static_cast<size_t>(HD / 16) * NT * 256;
+    static constexpr size_t kBytes = kSeen + 2 * kPairs * 4 + 16;
+    static constexpr int kBlocks = (HD * NT <= 256 ? 16 : HD * NT <= 384 ? 12 : 8) / kWarps;   // CTAs an SM that registers and shared memory leave room for
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -56,8 +68,23 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Codes in the high bytes of two halves -> two fp16 of value * 2^-8.
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u); }
+// Transposes an 8 x 8 matrix of 16-bit elements held as C fragments (lane (g, t): row g, columns 2t, 2t + 1).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// The two codes in the low (high) 16 bits as fp16, exactly.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(h) : "r"(w));
+    return h;
+}
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(h) : "r"(w));
+    return h;
+}
 
 // The rows of a tile: what the kernel and the join agree on.
 struct Rows {
@@ -97,14 +124,19 @@ struct Args {
     const uint32_t* qpos;
     uint16_t* y;
     float* part;
+    uint32_t* done;   // a counter per tile, zero between launches
     int* status;
     uint32_t rows, ldq, ldg, ldy, group, max_q, max_len, tiles, chunk, chunks;
-    float scale;      // hd^-1/2 log2(e) 2^8
+    float scale;      // hd^-1/2 log2(e)
 };
 
-// o, normalised -> gate, 16 bits. 8 values of hd columns d .. d + 7.
+// Columns d .. d + 7 of a pair: sums over the total, gate, 16 bits. A row that attends nothing has no total: zero.
 template <typename Act>
-__device__ __forceinline__ void store8(const Args& a, uint32_t row, uint32_t col, float (&o)[8]) {
+__device__ __forceinline__ void finish(const Args& a, const Rows& r, uint32_t pair, uint32_t kvh, uint32_t d, uint32_t hd, float total, float (&o)[8]) {
+    const uint32_t row = r.start + pair / a.group, col = (kvh * a.group + pair % a.group) * hd + d;
+    const float by = total == 0.f ? 0.f : 1.0f / total;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= by;
     if (a.gate) {
         const float4 g0 = *reinterpret_cast<const float4*>(a.gate + static_cast<size_t>(row) * a.ldg + col);
         const float4 g1 = *reinterpret_cast<const float4*>(a.gate + static_cast<size_t>(row) * a.ldg + col + 4);
@@ -116,19 +148,18 @@ __device__ __forceinline__ void store8(const Args& a, uint32_t row, uint32_t col
         make_uint4(Act::pack(o[0], o[1]), Act::pack(o[2], o[3]), Act::pack(o[4], o[5]), Act::pack(o[6], o[7]));
 }
 
-// One CTA: 16 (row, head) pairs of a sequence's kv head over one chunk of its keys. FEW: at most 8 pairs, whose weights go in
-// twice: rows 0..7 of the A operand hold them rounded to fp16 and rows 8..15 what the rounding left, so that the V product sees 22
-// bits of each weight at no extra instruction of the tensor cores.
-template <typename Act, int HD, bool FEW>
-__global__ void __launch_bounds__(kThreads, HD == 128 ? 4 : 2) kv8_attn_kernel(const Args a) {
-    using S = Shape<HD>;
+// One CTA: 8 NT (row, head) pairs of a sequence's kv head over one chunk of its keys.
+template <typename Act, int HD, int NT>
+__global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlocks) kv8_attn_kernel(const Args a) {
+    using S = Shape<HD, NT>;
+    constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
     constexpr int kKVec = HD / 64;         // vectors of a key a lane holds
     constexpr int kVVec = HD / 128;
-    extern __shared__ __align__(16) uint8_t smem[];
-    uint8_t* ring = smem;
-    uint4* qf = reinterpret_cast<uint4*>(smem + S::kRing);
-    uint32_t* seen = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kQ);   // [16] tokens that a pair attends
-    float* rank = reinterpret_cast<float*>(seen + 16);                      // [16] power of two that a pair's q was divided by
+    constexpr uint32_t kPairs = S::kPairs;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint2* qf = reinterpret_cast<uint2*>(smem + S::kQ);
+    uint32_t* seen = reinterpret_cast<uint32_t*>(smem + S::kSeen);   // tokens that a pair attends
+    float* rank = reinterpret_cast<float*>(seen + kPairs);           // power of two that a pair's q was divided by
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint32_t id = blockIdx.x;
@@ -139,87 +170,92 @@ __global__ void __launch_bounds__(kThreads, HD == 128 ? 4 : 2) kv8_attn_kernel(c
     id /= a.c.nkv;
     const uint32_t mt = id % a.tiles, j = id / a.tiles;
 
+    // The pages of the warp's tiles warp + kWarps i: lane i remembers that of tile i, 32 tiles at a time, and its scales. Where the last key
+    // is not known yet, the table is read ahead of it (never past its row).
+    const uint32_t key0 = z * a.chunk;
+    const uint32_t* table = a.c.table + static_cast<size_t>(j) * a.c.max_pages;
+    auto column = [&](uint32_t i) { return (key0 + (warp + kWarps * i) * kTile) / a.c.page_size; };
+    uint32_t page_ahead = column(lane) < a.c.max_pages ? table[column(lane)] : 0u;
     const Rows r = rows_of(a.c, a.q_start, j, a.rows, a.max_q);
     const bool reports = kvh == 0 && z == 0 && threadIdx.x == 0;
     if (!r.ok) {
         if (reports && mt == 0) kv8_flag(a.status, DC_STATUS_KV8_OFFSETS);
         return;
     }
-    constexpr uint32_t kPairs = FEW ? 8 : 16;
     const uint32_t pair0 = mt * kPairs, pairs = r.count * a.group;
     if (pair0 >= pairs) return;
     if (r.len > a.max_len) {
         if (reports && mt == 0) kv8_flag(a.status, DC_STATUS_KV8_LENGTH);
         return;
     }
-    if (warp == 0) {
-        uint32_t n = 0;
+    uint32_t n = 0;   // every warp: lane p looks at pair p
+    const bool on = lane < static_cast<int>(kPairs) && pair0 + lane < pairs;
+    {
         bool past = false;
-        if (lane < static_cast<int>(kPairs) && pair0 + lane < pairs) n = visible(r, a.qpos, (pair0 + lane) / a.group, &past);
-        if (lane < 16) seen[lane] = n;
-        if (past && kvh == 0 && z == 0) kv8_flag(a.status, DC_STATUS_KV8_POSITION);
+        if (on) n = visible(r, a.qpos, (pair0 + lane) / a.group, &past);
+        if (past && kvh == 0 && z == 0 && warp == 0) kv8_flag(a.status, DC_STATUS_KV8_POSITION);
     }
-    __syncthreads();
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(kPairs); ++i) most = max(most, seen[i]);
-    const uint32_t key0 = z * a.chunk;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, n), least = __reduce_min_sync(0xffffffffu, on ? n : 0xffffffffu);
     if (z && key0 >= most) return;
+    if (warp == 0 && lane < static_cast<int>(kPairs)) seen[lane] = n;
     const uint32_t key1 = min(most, key0 + a.chunk);
     const uint32_t tiles = (key1 - key0 + kTile - 1) / kTile;                     // of the CTA
     const uint32_t mine = tiles > static_cast<uint32_t>(warp) ? (tiles - warp + kWarps - 1) / kWarps : 0u;   // of the warp: tile warp + kWarps i
 
-    // lane i remembers page and scales of the warp's tile i
-    uint64_t page_at = 0;
-    float k_scale = 0.f, v_exp = 0.f;
-    if (static_cast<uint32_t>(lane) < mine) {
-        const uint32_t key = key0 + (warp + kWarps * lane) * kTile;
-        uint32_t page = a.c.table[static_cast<size_t>(j) * a.c.max_pages + key / a.c.page_size];
-        const bool inside = page < a.c.n_pages;
-        if (!inside) {
-            kv8_flag(a.status, DC_STATUS_KV8_PAGE);
-            page = 0;
+    uint64_t page_at = 0;                   // of the 32 tiles being fetched
+    float next_k = 0.f, next_v = 0.f;       // their scales
+    auto turn = [&](uint32_t i) {           // to tiles i .. i + 31
+        const uint32_t mine_i = i + lane, key = key0 + (warp + kWarps * mine_i) * kTile;
+        if (mine_i < mine) {
+            uint32_t page = i ? table[column(mine_i)] : page_ahead;
+            const bool inside = page < a.c.n_pages;
+            if (!inside) {
+                kv8_flag(a.status, DC_STATUS_KV8_PAGE);
+                page = 0;
+            }
+            page_at = page * a.c.page_stride + kvh * a.c.head_stride + (key % a.c.page_size) * a.c.token_stride;
+            next_k = a.c.k_scale[static_cast<size_t>(page) * a.c.nkv + kvh];
+            next_v = a.c.v_scale[static_cast<size_t>(page) * a.c.nkv + kvh];
+            if (!inside) next_k = __uint_as_float(0x7fffffffu);   // what attends it is NaN
         }
-        page_at = page * a.c.page_stride + kvh * a.c.head_stride + (key % a.c.page_size) * a.c.token_stride;
-        k_scale = a.c.k_scale[static_cast<size_t>(page) * a.c.nkv + kvh];
-        v_exp = kv8_log2i(a.c.v_scale[static_cast<size_t>(page) * a.c.nkv + kvh]);
-        if (!inside) k_scale = __uint_as_float(0x7fffffffu);   // what attends it is NaN
-    }
+    };
 
-    const uint8_t* kc = static_cast<const uint8_t*>(a.c.k);
-    const uint8_t* vc = static_cast<const uint8_t*>(a.c.v);
-    const uint32_t my_ring = smem_u32(ring) + warp * (S::kStages * S::kStage) + lane * 16;
-    auto fetch = [&](uint32_t i) {   // the warp's tile i; every lane runs this
-        const uint64_t at = __shfl_sync(0xffffffffu, page_at, i & 31);
-        uint32_t dst = my_ring + (i % S::kStages) * S::kStage;
-        const uint8_t* ks = kc + at + 16 * t;
+    // A warp copies kRows rows of HD codes an instruction.
+    constexpr int kRows = 512 / HD, kPieces = HD / 16;
+    const uint32_t token = static_cast<uint32_t>(a.c.token_stride);
+    const uint32_t fill_row = lane / kPieces, piece = lane % kPieces;
+    const uint8_t* kc = static_cast<const uint8_t*>(a.c.k) + fill_row * token + 16 * piece;
+    const uint8_t* vc = static_cast<const uint8_t*>(a.c.v) + fill_row * token + 16 * piece;
+    const uint8_t* ring = smem + warp * (S::kStages * S::kStage);
+    const uint32_t fill_k = smem_u32(ring) + fill_row * HD + 16 * (piece ^ (4 * (fill_row & 1))), fill_v = smem_u32(ring) + 16 * HD + fill_row * HD + 16 * (piece ^ (fill_row & 6));
+    auto fetch = [&](uint32_t i, uint32_t stage) {   // the warp's tile i; every lane runs this
+        if (i % 32 == 0) turn(i);
+        const uint64_t at = __shfl_sync(0xffffffffu, page_at, i % 32);
+        const uint32_t to = stage * static_cast<uint32_t>(S::kStage);
+        const uint8_t *ks = kc + at, *vs = vc + at;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int v = 0; v < kKVec; ++v, dst += 512) cp16(dst, ks + (g + 8 * n) * a.c.token_stride + 64 * v);
-        const uint8_t* vs = vc + at + 16 * g;
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-            for (int v = 0; v < kVVec; ++v, dst += 512) cp16(dst, vs + (2 * t + (p & 1) + 8 * (p >> 1)) * a.c.token_stride + 128 * v);
+        for (int n = 0; n < 16 / kRows; ++n, ks += kRows * token, vs += kRows * token) {
+            cp16(fill_k + to + n * 512, ks);
+            cp16((fill_v ^ (16 * (n * kRows & 6))) + to + n * 512, vs);
+        }
     };
 #pragma unroll
     for (int i = 0; i + 1 < S::kStages; ++i) {
-        if (static_cast<uint32_t>(i) < mine) fetch(i);
+        if (static_cast<uint32_t>(i) < mine) fetch(i, i);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    // q as A fragments, in the order that the K codes lie in: k-step 4 v + w of lane (g, t) takes hd 64 v + 16 t + 4 w + {0, 2 | 1, 3}.
-    // A bf16 row is first divided by a power of two that brings its largest magnitude to [2^14, 2^15): then its 8 bits fit fp16 but
-    // for elements 2^-28 below it. fp16 rows go in as they are.
-    for (uint32_t p = warp; p < 16; p += kWarps) {
-        const bool on = p < kPairs && pair0 + p < pairs;
+    // q as B fragments, in the order that the K codes lie in: k-step 4 v + w of lane (g, t) takes hd 64 v + 16 t + 4 w + {0, 1 | 2, 3}, 8 bytes
+    // of q as they are. A bf16 row is first divided by a power of two that brings its largest magnitude to [2^14, 2^15): then its 8
+    // bits fit fp16 but for elements 2^-28 below it. fp16 rows go in as they are.
+    for (uint32_t p = warp; p < kPairs; p += kWarps) {
+        const bool there = pair0 + p < pairs;
         const uint32_t row = r.start + (pair0 + p) / a.group, h = kvh * a.group + (pair0 + p) % a.group;
         const uint16_t* src = a.q + static_cast<size_t>(row) * a.ldq + static_cast<size_t>(h) * HD;
         constexpr int kWords = HD / 128;   // 8-byte pieces a lane holds: piece lane + 32 i is hd 4 (lane + 32 i) ..
         uint2 x[kWords];
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) x[i] = on ? *reinterpret_cast<const uint2*>(src + 4 * (lane + 32 * i)) : make_uint2(0, 0);
+        for (int i = 0; i < kWords; ++i) x[i] = there ? *reinterpret_cast<const uint2*>(src + 4 * (lane + 32 * i)) : make_uint2(0, 0);
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < kWords; ++i) top = __vmaxu2(top, __vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu));
@@ -243,237 +279,307 @@ __global__ void __launch_bounds__(kThreads, HD == 128 ? 4 : 2) kv8_attn_kernel(c
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
             const uint32_t hd = 4 * (lane + 32 * i), step = hd / 64 * 4 + hd % 16 / 4, to = hd % 64 / 16;   // to: t of the lane it belongs to
-            uint32_t* f = reinterpret_cast<uint32_t*>(qf + step * 32 + (p & 7) * 4 + to);
-            f[p >> 3] = (x[i].x & 0xffffu) | (x[i].y << 16);                 // hd + 0, hd + 2: k = 2t, 2t + 1
-            f[2 + (p >> 3)] = (x[i].x >> 16) | (x[i].y & 0xffff0000u);       // hd + 1, hd + 3: k = 2t + 8, 2t + 9
+            qf[(step * NT + (p >> 3)) * 32 + (p & 7) * 4 + to] = x[i];
         }
     }
     __syncthreads();
 
-    const uint32_t see0 = seen[g], see1 = seen[FEW ? g : g + 8];
-    const float mul0 = a.scale * rank[g], mul1 = FEW ? 0.f : a.scale * rank[g + 8];
-    float o[HD / 8][4];
+    // pairs 8 n + 2 t and + 1 of each tile of pairs: the columns of this lane's C fragments
+    float mul[NT][2], m[NT][2], l[NT][2];
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i)
+    for (int b = 0; b < NT; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m0 = kNone, m1 = kNone, l0 = 0.f, l1 = 0.f;
+        for (int e = 0; e < 2; ++e) {
+            mul[b][e] = a.scale * rank[8 * b + 2 * t + e];
+            m[b][e] = kNone;
+            l[b][e] = 0.f;
+        }
+    constexpr bool kKeepQ = NT * HD <= 128;   // q fragments in registers where there is room
+    uint2 q_kept[kKeepQ ? HD / 16 : 1];
+    if (kKeepQ) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) q_kept[kKeepQ ? i : 0] = qf[i * 32 + lane];
+    }
+    float o[NT][HD / 16][4];
+#pragma unroll
+    for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[b][d][e] = 0.f;
 
+    const uint32_t read_k0 = g * HD + 16 * (t + 4 * (g & 1)), read_k1 = read_k0 ^ 64, read_v = 16 * HD + 2 * t * HD + 16 * (g ^ (2 * t));
+    uint32_t stage = 0;
+    float k_scale = 0.f, v_scale = 0.f;   // of the 32 tiles being worked on
     for (uint32_t i = 0; i < mine; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-        const uint8_t* at = ring + warp * (S::kStages * S::kStage) + (i % S::kStages) * S::kStage + lane * 16;
-        float s[2][4];
+        __syncwarp();   // all lanes' copies of this stage have landed, and all have read the stage that is filled next
+        if (i % 32 == 0) k_scale = next_k, v_scale = next_v;
+        const uint8_t* at = ring + stage * S::kStage;
+        const uint32_t key = key0 + (warp + kWarps * i) * kTile;
+        float s[NT][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        for (int b = 0; b < NT; ++b) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
 #pragma unroll
-            for (int v = 0; v < kKVec; ++v) {
-                const uint4 x = *reinterpret_cast<const uint4*>(at + (n * kKVec + v) * 512);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int v = 0; v < kKVec; ++v) {
+            const uint8_t* from = at + (v & 1 ? read_k1 : read_k0) + 128 * (v >> 1);
+            const uint4 x = *reinterpret_cast<const uint4*>(from), y = *reinterpret_cast<const uint4*>(from + 8 * HD);
+            const uint32_t w0[4] = {x.x, x.y, x.z, x.w}, w1[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint4 f = qf[(4 * v + e) * 32 + lane];
-                    mma_f16(s[n], f.x, f.y, f.z, f.w, high_codes(w[e] << 8), high_codes(w[e]));
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t a0 = low_codes(w0[e]), a1 = low_codes(w1[e]), a2 = high_codes(w0[e]), a3 = high_codes(w1[e]);
+#pragma unroll
+                for (int b = 0; b < NT; ++b) {
+                    const uint2 f = kKeepQ ? q_kept[kKeepQ ? 4 * v + e : 0] : qf[((4 * v + e) * NT + b) * 32 + lane];
+                    mma_f16(s[b], a0, a1, a2, a3, f.x, f.y);
                 }
             }
         }
-        const float ks = __shfl_sync(0xffffffffu, k_scale, i & 31);
-        float ve = __shfl_sync(0xffffffffu, v_exp, i & 31);
+        const float ks = __shfl_sync(0xffffffffu, k_scale, i % 32), ve = kv8_log2i(__shfl_sync(0xffffffffu, v_scale, i % 32));
         const float back = isnan(ve) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(ve))));   // 2^-e_v; a NaN reaches the sum through the weights
-        const uint32_t key = key0 + (warp + kWarps * i) * kTile + 2 * t;
-        const float c0 = mul0 * ks, c1 = mul1 * ks;
+        bool grow = false;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                s[n][e] = key + 8 * n + e < see0 ? fmaf(s[n][e], c0, ve) : -INFINITY;
-                if (!FEW) s[n][2 + e] = key + 8 * n + e < see1 ? fmaf(s[n][2 + e], c1, ve) : -INFINITY;
-            }
-        const float top0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-        const float top1 = FEW ? -INFINITY : fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-        if (__any_sync(0xffffffffu, top0 > m0 + kStep || (!FEW && top1 > m1 + kStep))) {
-            // the four lanes of a row agree on the new maximum; rows whose maximum stays put scale by 1
-            float n0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
-            n0 = fmaxf(m0, fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2)));
-            const float by0 = ex2(m0 - n0);
-            m0 = n0;
-            l0 *= by0;
-            float by1 = by0;
-            if (!FEW) {
-                float n1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
-                n1 = fmaxf(m1, fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2)));
-                by1 = ex2(m1 - n1);
-                m1 = n1;
-                l1 *= by1;
-            }
-#pragma unroll
-            for (int d = 0; d < HD / 8; ++d) {
-                o[d][0] *= by0;
-                o[d][1] *= by0;
-                o[d][2] *= by1;
-                o[d][3] *= by1;
-            }
-        }
-        float p[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int b = 0; b < NT; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                p[n][e] = ex2(s[n][e] - m0);
-                l0 = fmaf(p[n][e], back, l0);
-                if (!FEW) {
-                    p[n][2 + e] = ex2(s[n][2 + e] - m1);
-                    l1 = fmaf(p[n][2 + e], back, l1);
+                const float by = mul[b][e] * ks;
+                s[b][e] = fmaf(s[b][e], by, ve);
+                s[b][2 + e] = fmaf(s[b][2 + e], by, ve);
+            }
+        if (key + kTile > least) {   // some pair does not see all of the tile
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t see = seen[8 * b + 2 * t + e];
+                    if (key + g >= see) s[b][e] = -INFINITY;
+                    if (key + g + 8 >= see) s[b][2 + e] = -INFINITY;
                 }
-            }
-        const uint32_t a0 = ActF16::pack(p[0][0], p[0][1]), a2 = ActF16::pack(p[1][0], p[1][1]);
-        uint32_t a1, a3;
-        if (FEW) {
-            a1 = ActF16::pack(p[0][0] - ActF16::lo(a0), p[0][1] - ActF16::hi(a0));
-            a3 = ActF16::pack(p[1][0] - ActF16::lo(a2), p[1][1] - ActF16::hi(a2));
-        } else {
-            a1 = ActF16::pack(p[0][2], p[0][3]);
-            a3 = ActF16::pack(p[1][2], p[1][3]);
+        }
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[b][e], s[b][2 + e]) > m[b][e] + kStep;
+        if (__any_sync(0xffffffffu, grow)) {
+            // the eight lanes of a pair agree on the new maximum; pairs whose maximum stays put scale by 1
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[b][e], s[b][2 + e]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(m[b][e], fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)));
+                    const float by = ex2(m[b][e] - top);
+                    m[b][e] = top;
+                    l[b][e] *= by;
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d) {
+                        o[b][d][e] *= by;
+                        o[b][d][2 + e] *= by;
+                    }
+                }
+        }
+        uint32_t p0[NT], p1[NT];   // B fragments of the weights
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            const float w00 = ex2(s[b][0] - m[b][0]), w01 = ex2(s[b][1] - m[b][1]), w10 = ex2(s[b][2] - m[b][0]), w11 = ex2(s[b][3] - m[b][1]);
+            l[b][0] = fmaf(w00 + w10, back, l[b][0]);
+            l[b][1] = fmaf(w01 + w11, back, l[b][1]);
+            p0[b] = transpose8(ActF16::pack(w00, w01));
+            p1[b] = transpose8(ActF16::pack(w10, w11));
         }
 #pragma unroll
         for (int v = 0; v < kVVec; ++v) {
             uint32_t x[4][4];
 #pragma unroll
-            for (int p4 = 0; p4 < 4; ++p4) {
-                const uint4 u = *reinterpret_cast<const uint4*>(at + (2 * kKVec + p4 * kVVec + v) * 512);
-                x[p4][0] = u.x, x[p4][1] = u.y, x[p4][2] = u.z, x[p4][3] = u.w;
+            for (int p = 0; p < 4; ++p) {
+                const uint4 u = *reinterpret_cast<const uint4*>(at + read_v + ((p & 1) + 8 * (p >> 1)) * HD + 128 * v);
+                x[p][0] = u.x, x[p][1] = u.y, x[p][2] = u.z, x[p][3] = u.w;
+            }
+            if (key + kTile > r.len) {   // what lies behind the last token
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                    if (key + 2 * t + (p & 1) + 8 * (p >> 1) >= r.len) x[p][0] = x[p][1] = x[p][2] = x[p][3] = 0u;
             }
 #pragma unroll
-            for (int b = 0; b < 16; ++b) {
-                // byte b % 4 of two keys' words into the high bytes of two halves
-                const uint32_t pick = ((b & 3) << 4) | ((4 + (b & 3)) << 12);
-                mma_f16(o[16 * v + b], a0, a1, a2, a3, high_codes(__byte_perm(x[0][b >> 2], x[1][b >> 2], pick)),
-                        high_codes(__byte_perm(x[2][b >> 2], x[3][b >> 2], pick)));
+            for (int d = 0; d < 8; ++d) {   // columns 2 d and 2 d + 1 of the lane's 16
+                const uint32_t pick = d & 1 ? 0x7362u : 0x5140u;   // bytes 0, 1 or 2, 3 of two keys' words, key by key
+                const uint32_t w0 = __byte_perm(x[0][d >> 1], x[1][d >> 1], pick), w1 = __byte_perm(x[2][d >> 1], x[3][d >> 1], pick);
+                const uint32_t a0 = low_codes(w0), a1 = high_codes(w0), a2 = low_codes(w1), a3 = high_codes(w1);
+#pragma unroll
+                for (int b = 0; b < NT; ++b) mma_f16(o[b][8 * v + d], a0, a1, a2, a3, p0[b], p1[b]);
             }
         }
-        if (i + S::kStages - 1 < mine) fetch(i + S::kStages - 1);
+        const uint32_t next = stage == 0 ? S::kStages - 1 : stage - 1;   // (i + kStages - 1) % kStages
+        if (i + S::kStages - 1 < mine) fetch(i + S::kStages - 1, next);
         asm volatile("cp.async.commit_group;" ::: "memory");
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 
-    // the four lanes of a row add their sums; the warps' partial results meet in shared memory
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    __syncthreads();   // the ring and the q fragments are free
-    constexpr int kLd = HD + 2;
-    float* mine_at = reinterpret_cast<float*>(smem) + warp * (kPairs * kLd);
-    if (t == 0) {
-        mine_at[g * kLd + HD] = m0;
-        mine_at[g * kLd + HD + 1] = l0;
-        if (!FEW) {
-            mine_at[(g + 8) * kLd + HD] = m1;
-            mine_at[(g + 8) * kLd + HD + 1] = l1;
-        }
-    }
+    // the eight lanes of a pair add their totals; the warps' partial results meet in shared memory
+    __syncthreads();   // the ring is free
+    float* mine_at = reinterpret_cast<float*>(smem) + warp * (kPairs * S::kLd);
 #pragma unroll
-    for (int v = 0; v < kVVec; ++v)
+    for (int b = 0; b < NT; ++b)
 #pragma unroll
-        for (int b = 0; b < 16; ++b) {
-            const int d = 128 * v + 32 * t + b;
-            const float (&x)[4] = o[16 * v + b];
-            mine_at[g * kLd + d] = FEW ? x[0] + x[2] : x[0];
-            mine_at[g * kLd + d + 16] = FEW ? x[1] + x[3] : x[1];
-            if (!FEW) {
-                mine_at[(g + 8) * kLd + d] = x[2];
-                mine_at[(g + 8) * kLd + d + 16] = x[3];
-            }
+        for (int e = 0; e < 2; ++e) {
+            float total = l[b][e];
+            total += __shfl_xor_sync(0xffffffffu, total, 4);
+            total += __shfl_xor_sync(0xffffffffu, total, 8);
+            total += __shfl_xor_sync(0xffffffffu, total, 16);
+            float* to = mine_at + (8 * b + 2 * t + e) * S::kLd;
+            if (g == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m[b][e], total);
+#pragma unroll
+            for (int v = 0; v < kVVec; ++v)
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    *reinterpret_cast<float4*>(to + 128 * v + 16 * g + 4 * d) =
+                        make_float4(o[b][8 * v + 2 * d][e], o[b][8 * v + 2 * d][2 + e], o[b][8 * v + 2 * d + 1][e], o[b][8 * v + 2 * d + 1][2 + e]);
         }
     __syncthreads();
     const float* all = reinterpret_cast<const float*>(smem);
     const bool whole = most <= a.chunk;   // this CTA has seen every key
-    for (uint32_t e = threadIdx.x; e < kPairs * (HD / 8); e += kThreads) {
+    float* parts = a.part + static_cast<size_t>(tile_id) * a.chunks * (kPairs * S::kLd);
+    const uint32_t here = min(kPairs, pairs - pair0);
+    for (uint32_t e = threadIdx.x; e < here * (HD / 8); e += kThreads) {
         const uint32_t p = e / (HD / 8), d = e % (HD / 8) * 8;
-        if (pair0 + p >= pairs) continue;
-        float m = kNone, l = 0.f, x[8] = {};
+        float top = kNone, total = 0.f, x[8] = {};
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, all[(w * kPairs + p) * kLd + HD]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, all[(w * kPairs + p) * S::kLd + HD]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float* from = all + (w * kPairs + p) * kLd;
-            const float by = ex2(from[HD] - m);
-            l = fmaf(from[HD + 1], by, l);
+            const float* from = all + (w * kPairs + p) * S::kLd;
+            const float by = ex2(from[HD] - top);
+            total = fmaf(from[HD + 1], by, total);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(from[d + i], by, x[i]);
         }
         if (whole) {
-            const float by = l == 0.f ? 0.f : 256.f / l;   // a row that attends nothing
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= by;
-            store8<Act>(a, r.start + (pair0 + p) / a.group, (kvh * a.group + (pair0 + p) % a.group) * HD + d, x);
+            finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
         } else {
-            float* to = a.part + ((static_cast<size_t>(tile_id) * a.chunks + z) * kPairs + p) * (HD + 4);
+            float* to = parts + (z * kPairs + p) * S::kLd;
             *reinterpret_cast<float4*>(to + d) = make_float4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<float4*>(to + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m, l);
+            if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(top, total);
         }
     }
-}
+    if (whole) return;
 
-// Joins the chunks of a tile's pairs, in chunk order. One CTA a tile; tiles that one chunk held have written their rows already.
-template <typename Act, int HD>
-__global__ void __launch_bounds__(256) kv8_join_kernel(const Args a, uint32_t per_tile) {
-    uint32_t id = blockIdx.x;
-    const uint32_t tile_id = id, kvh = id % a.c.nkv;
-    id /= a.c.nkv;
-    const uint32_t mt = id % a.tiles, j = id / a.tiles;
-    const Rows r = rows_of(a.c, a.q_start, j, a.rows, a.max_q);
-    if (!r.ok || r.len > a.max_len) return;
-    const uint32_t pair0 = mt * per_tile, pairs = r.count * a.group;
-    if (pair0 >= pairs) return;
-    uint32_t most = 0;
-    bool past = false;
-    if ((threadIdx.x & 31) < per_tile && pair0 + (threadIdx.x & 31) < pairs) most = visible(r, a.qpos, (pair0 + (threadIdx.x & 31)) / a.group, &past);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (most <= a.chunk) return;
+    // The last of the tile's CTAs joins the chunks. Threads take 8 columns of a pair; where that leaves threads over they share the chunks
+    // (`groups` of them, chunk k with group k % groups), and the groups' sums are added in order.
     const uint32_t chunks = (most + a.chunk - 1) / a.chunk;
-    const size_t step = static_cast<size_t>(per_tile) * (HD + 4);
-    for (uint32_t e = threadIdx.x; e < per_tile * (HD / 8); e += 256) {
-        const uint32_t p = e / (HD / 8), d = e % (HD / 8) * 8;
-        if (pair0 + p >= pairs) continue;
-        const float* from = a.part + (static_cast<size_t>(tile_id) * a.chunks * per_tile + p) * (HD + 4);
-        float m = kNone, l = 0.f, x[8] = {};
-        for (uint32_t z = 0; z < chunks; ++z) m = fmaxf(m, from[z * step + HD]);
-        for (uint32_t z = 0; z < chunks; ++z) {
-            const float2 ml = *reinterpret_cast<const float2*>(from + z * step + HD);
-            const float4 u = *reinterpret_cast<const float4*>(from + z * step + d), w = *reinterpret_cast<const float4*>(from + z * step + d + 4);
-            const float by = ex2(ml.x - m), v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-            l = fmaf(ml.y, by, l);
+    uint32_t* last = reinterpret_cast<uint32_t*>(smem + S::kSeen + 2 * kPairs * 4);
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) *last = atomicInc(a.done + tile_id, chunks - 1) == chunks - 1;   // the last arrival leaves 0
+    __syncthreads();
+    if (!*last) return;
+    __threadfence();
+    constexpr uint32_t kCols = HD / 8;
+    const uint32_t items = here * kCols;
+    const uint32_t groups = items >= kThreads ? 1u : kThreads / items, group = groups == 1 ? 0u : threadIdx.x / items;
+    float* sums = reinterpret_cast<float*>(smem);   // [groups][here][kLd]
+    for (uint32_t e = groups == 1 ? threadIdx.x : threadIdx.x % items; e < items && group < groups; e += kThreads) {
+        const uint32_t p = e / kCols, d = e % kCols * 8;
+        const float* from = parts + p * S::kLd;
+        float top = kNone, total = 0.f, x[8] = {};
+        for (uint32_t k0 = group; k0 < chunks; k0 += 4 * groups) {   // four chunks' loads in flight
+            float2 ml[4];
+            float4 u[4], w[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = fmaf(v[i], by, x[i]);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t k = k0 + i * groups;
+                const float* at = from + static_cast<size_t>(min(k, chunks - 1)) * (kPairs * S::kLd);
+                ml[i] = __ldcg(reinterpret_cast<const float2*>(at + HD));
+                u[i] = __ldcg(reinterpret_cast<const float4*>(at + d));
+                w[i] = __ldcg(reinterpret_cast<const float4*>(at + d + 4));
+                if (k >= chunks) ml[i] = make_float2(kNone, 0.f), u[i] = w[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            const float now = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), old = ex2(top - now);
+            top = now;
+            total *= old;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= old;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float by = ex2(ml[i].x - now), v[8] = {u[i].x, u[i].y, u[i].z, u[i].w, w[i].x, w[i].y, w[i].z, w[i].w};
+                total = fmaf(ml[i].y, by, total);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) x[c] = fmaf(v[c], by, x[c]);
+            }
         }
-        const float by = l == 0.f ? 0.f : 256.f / l;
+        if (groups == 1) {
+            finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
+        } else {
+            float* to = sums + (group * here + p) * S::kLd;
+            *reinterpret_cast<float4*>(to + d) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(to + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(top, total);
+        }
+    }
+    if (groups == 1) return;
+    __syncthreads();
+    if (threadIdx.x < items) {
+        const uint32_t p = threadIdx.x / kCols, d = threadIdx.x % kCols * 8;
+        float top = kNone, total = 0.f, x[8] = {};
+        for (uint32_t k = 0; k < groups; ++k) top = fmaxf(top, sums[(k * here + p) * S::kLd + HD]);
+        for (uint32_t k = 0; k < groups; ++k) {
+            const float* at = sums + (k * here + p) * S::kLd;
+            const float by = ex2(at[HD] - top);
+            total = fmaf(at[HD + 1], by, total);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= by;
-        store8<Act>(a, r.start + (pair0 + p) / a.group, (kvh * a.group + (pair0 + p) % a.group) * HD + d, x);
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(at[d + i], by, x[i]);
+        }
+        finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
     }
 }
 
-// How a call is cut: tiles of `pairs` (row, head) pairs, chunks of `chunk` keys.
+typedef void (*attn_fn)(const Args);
+struct Variant {
+    attn_fn f;
+    int bytes, threads, blocks;
+};
+template <typename Act>
+Variant pick(uint32_t hd, uint32_t nt) {
+#define DC_KV8_VARIANT(HD, NT) Variant{kv8_attn_kernel<Act, HD, NT>, static_cast<int>(Shape<HD, NT>::kBytes), Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlocks}
+    if (hd == 128) return nt == 1 ? DC_KV8_VARIANT(128, 1) : DC_KV8_VARIANT(128, 2);
+    return nt == 1 ? DC_KV8_VARIANT(256, 1) : DC_KV8_VARIANT(256, 2);
+#undef DC_KV8_VARIANT
+}
+
+// How a call is cut: tiles of 8 nt (row, head) pairs, chunks of `chunk` keys.
+constexpr uint64_t kDoneCounters = DC_KV8_DONE_COUNTERS;
 struct Cut {
-    uint32_t pairs, tiles, max_len, chunk, chunks;
+    uint32_t nt, tiles, max_len, chunk, chunks;
     uint64_t ctas;
 };
 Cut cut_of(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
     Cut t;
-    const uint32_t group = nq / c->nkv;
-    const uint64_t pairs = static_cast<uint64_t>(max_q) * group;
-    t.pairs = pairs <= 8 ? 8 : 16;
-    t.tiles = static_cast<uint32_t>((pairs + t.pairs - 1) / t.pairs);
+    // Pairs in eights, a CTA each: many narrow tiles hide their latencies better than few wide ones (24 pairs over 2,307 keys: 10.0 us in
+    // eights, 12.1 in sixteens), until the tiles alone are more than the GPU holds at once; then two eights share a pass over the codes
+    // (16 pairs of 64 x 1,200 keys: 44 against 52 us).
+    const uint64_t eights = (static_cast<uint64_t>(max_q) * (nq / c->nkv) + 7) / 8;
     const uint32_t cap = c->max_pages * c->page_size;
     const uint32_t len = max_len == 0 || max_len > cap ? cap : max_len;
-    const uint64_t whole = static_cast<uint64_t>(c->n_seqs) * c->nkv * t.tiles;
-    // Chunks as long as they can be while there are about six CTAs an SM to balance the load with, from 256 to kMaxChunk keys.
-    const uint64_t want = (static_cast<uint64_t>(ctx->sm_count) * 6 + whole - 1) / whole;
-    uint64_t chunk = (len + want - 1) / want;
-    chunk = (chunk + 127) / 128 * 128;
-    t.chunk = static_cast<uint32_t>(chunk < 256 ? 256 : chunk > kMaxChunk ? kMaxChunk : chunk);
+    const uint64_t items = static_cast<uint64_t>(c->n_seqs) * c->nkv;
+    Variant v = pick<dc::ActF16>(c->hd, 1);
+    t.nt = eights > 1 && items * eights > static_cast<uint64_t>(ctx->sm_count) * v.blocks ? 2 : 1;
+    v = pick<dc::ActF16>(c->hd, t.nt);
+    t.tiles = static_cast<uint32_t>((eights + t.nt - 1) / t.nt);
+    const uint64_t whole = items * t.tiles;
+    const uint32_t warps = v.threads / 32, step = warps * kTile;   // a tile for each warp
+    // Chunks. A join costs about 3 us and 0.1 us a chunk, a tile 0.5 us of its warp's time: keys of up to five tiles a warp stay whole
+    // (603 keys of one request: 7.2 us whole, 7.7 cut in 10), others are cut in about sqrt(tiles of a warp * HD / 32), as long as every
+    // SM has at most one set of eight warps to run (16,000 keys: 12.7 us in 18 chunks, 16.0 in 31; 131,071: 52.2 in 18, 54.4 in 37).
+    uint64_t parts = 1;
+    if (len > 5 * step && whole <= kDoneCounters) {
+        const uint64_t room = static_cast<uint64_t>(ctx->sm_count) * 8 / warps / whole;
+        parts = static_cast<uint64_t>(sqrt(static_cast<double>(len) / kTile * c->hd / 32 / warps));
+        if (parts > room) parts = room < 1 ? 1 : room;
+    }
+    t.chunk = static_cast<uint32_t>(((len + parts - 1) / parts + step - 1) / step * step);
     t.max_len = len;
     t.chunks = (len + t.chunk - 1) / t.chunk;
     t.ctas = whole * t.chunks;
@@ -481,14 +587,7 @@ Cut cut_of(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q
 }
 size_t part_bytes(const dc_kv8_cache* c, const Cut& t) {
     if (t.chunks <= 1) return 0;
-    return static_cast<size_t>(t.ctas) * t.pairs * (c->hd + 4) * sizeof(float);
-}
-
-typedef void (*attn_fn)(const Args);
-template <typename Act>
-attn_fn pick(uint32_t hd, bool few) {
-    if (hd == 128) return few ? kv8_attn_kernel<Act, 128, true> : kv8_attn_kernel<Act, 128, false>;
-    return few ? kv8_attn_kernel<Act, 256, true> : kv8_attn_kernel<Act, 256, false>;
+    return static_cast<size_t>(t.ctas) * 8 * t.nt * (c->hd + 4) * sizeof(float);
 }
 
 }  // namespace
@@ -496,12 +595,11 @@ attn_fn pick(uint32_t hd, bool few) {
 int dc_kv8_attention_warm(dc_ctx* ctx) {
     static bool set[16] = {};
     if (set[ctx->device & 15]) return DC_OK;
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t hd = i & 1 ? 256 : 128;
-        const attn_fn f = i & 4 ? pick<dc::ActF16>(hd, i & 2) : pick<dc::ActBF16>(hd, i & 2);
-        const int bytes = static_cast<int>(hd == 128 ? Shape<128>::kBytes : Shape<256>::kBytes);
-        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != cudaSuccess) return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention: cannot opt in to %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t hd = i & 1 ? 256 : 128, nt = 1 + (i >> 1 & 3);
+        const Variant v = i & 8 ? pick<dc::ActF16>(hd, nt) : pick<dc::ActBF16>(hd, nt);
+        const cudaError_t e = cudaFuncSetAttribute(v.f, cudaFuncAttributeMaxDynamicSharedMemorySize, v.bytes);
+        if (e != cudaSuccess) return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention: cannot opt in to %d bytes of shared memory: %s", v.bytes, cudaGetErrorString(e));
     }
     set[ctx->device & 15] = true;
     return DC_OK;
@@ -540,6 +638,7 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     a.c.k_scale = cache->k_scale + static_cast<size_t>(layer) * cache->n_pages * cache->nkv;
     a.c.v_scale = cache->v_scale + static_cast<size_t>(layer) * cache->n_pages * cache->nkv;
     a.part = nullptr;
+    a.done = ctx->kv8_done;
     if (t.chunks > 1) {
         void* ws = nullptr;
         if ((rc = dc_get_workspace(ctx, part_bytes(cache, t), "kv8_attention", &ws)) != DC_OK) return rc;
@@ -554,14 +653,10 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     a.status = ctx->status_dev;
     a.rows = rows, a.ldq = ldq, a.ldg = ldg, a.ldy = ldy, a.group = nq / cache->nkv, a.max_q = most, a.max_len = t.max_len;
     a.tiles = t.tiles, a.chunk = t.chunk, a.chunks = t.chunks;
-    a.scale = 256.f * kLog2e / sqrtf(static_cast<float>(cache->hd));
+    a.scale = kLog2e / sqrtf(static_cast<float>(cache->hd));
     const bool f16 = ctx->act_dtype == DC_ACT_F16;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const attn_fn f = f16 ? pick<dc::ActF16>(cache->hd, t.pairs == 8) : pick<dc::ActBF16>(cache->hd, t.pairs == 8);
-    f<<<static_cast<uint32_t>(t.ctas), kThreads, cache->hd == 128 ? Shape<128>::kBytes : Shape<256>::kBytes, s>>>(a);
-    if ((rc = dc_check_launch(ctx, "kv8_attention")) != DC_OK || t.chunks == 1) return rc;
-    auto join = cache->hd == 128 ? (f16 ? kv8_join_kernel<dc::ActF16, 128> : kv8_join_kernel<dc::ActBF16, 128>)
-                                 : (f16 ? kv8_join_kernel<dc::ActF16, 256> : kv8_join_kernel<dc::ActBF16, 256>);
-    join<<<static_cast<uint32_t>(t.ctas / t.chunks), 256, 0, s>>>(a, t.pairs);
-    return dc_check_launch(ctx, "kv8_attention (join)");
+    const Variant v = f16 ? pick<dc::ActF16>(cache->hd, t.nt) : pick<dc::ActBF16>(cache->hd, t.nt);
+    v.f<<<static_cast<uint32_t>(t.ctas), v.threads, v.bytes, s>>>(a);
+    return dc_check_launch(ctx, "kv8_attention");
 }

@@ -393,6 +393,7 @@ extern "C" int dc_kv8_check(const dc_kv8_cache* c, char* err, size_t err_len) {
     if (c->n_seqs > 65535 || c->nkv > 1024 || c->layers > 65535) return fail_text(err, err_len, DC_UNSUPPORTED, "at most 65535 sequences, 65535 layers and 1024 kv heads");
     if (c->n_pages > 0x200000u) return fail_text(err, err_len, DC_UNSUPPORTED, "at most 2^21 pages");
     if (static_cast<uint64_t>(c->max_pages) * c->page_size >= 0x80000000ull) return fail_text(err, err_len, DC_UNSUPPORTED, "max_pages * page_size must be below 2^31");
+    if (c->token_stride >= (1ull << 28)) return fail_text(err, err_len, DC_UNSUPPORTED, "token_stride must be below 2^28");
     if (c->reserved) return fail_text(err, err_len, DC_INVALID_ARG, "reserved must be 0");
     // codes must not share bytes: going up by stride, each step clears all that lies within the smaller ones
     uint64_t stride[4] = {c->token_stride, c->head_stride, c->page_stride, c->layer_stride}, count[4] = {c->page_size, c->nkv, c->n_pages, c->layers};

@@ -393,7 +393,7 @@ typedef struct dc_kv8_cache {
 #define DC_KV8_NO_KEYS 0xFFFFFFFFu
 
 /* Checks the description alone (pointers set and aligned, page_size 16 | 32 | 64 | 128, hd 128 | 256, strides that keep
- * codes apart, n_seqs <= 65535, n_pages <= 2^21, max_pages * page_size < 2^31): DC_OK, or DC_INVALID_ARG / DC_UNSUPPORTED with a message in
+ * codes apart, token_stride < 2^28, n_seqs <= 65535, n_pages <= 2^21, max_pages * page_size < 2^31): DC_OK, or DC_INVALID_ARG / DC_UNSUPPORTED with a message in
  * `err` (may be NULL). Needs no GPU and no context. Every dc_kv8_* entry point makes the same checks. */
 int dc_kv8_check(const dc_kv8_cache* cache, char* err, size_t err_len);
 

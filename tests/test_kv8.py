@@ -67,6 +67,7 @@ def _struct(**changes):
     ({"hd": 64}, 3, "hd"), ({"page_size": 48}, 3, "page_size"), ({"page_size": 256}, 3, "page_size"), ({"nkv": 0}, 1, "at least 1"), ({"n_seqs": 0}, 1, "at least 1"),
     ({"max_pages": 0}, 1, "at least 1"), ({"n_seqs": 65536}, 3, "65535"), ({"n_pages": 0x200001, "layers": 1}, 3, "2^21"),
     ({"max_pages": 1 << 27}, 3, "2^31"), ({"reserved": 1}, 1, "reserved"), ({"token_stride": 136}, 1, "multiples"), ({"token_stride": 64}, 1, "overlap"),
+    ({"token_stride": 1 << 28, "layers": 1, "n_pages": 1, "nkv": 1}, 3, "2^28"),
     ({"page_stride": 7 * 16 * 128}, 1, "overlap"), ({"head_stride": 0}, 1, "overlap"), ({"layer_stride": 1 << 47, "layers": 65535}, 1, "2^48"),
     # the same bytes with a token's heads side by side, and a view with holes
     ({"head_stride": 128, "token_stride": 8 * 128}, 0, ""), ({"token_stride": 256, "head_stride": 32 * 128, "page_stride": 1 << 20, "layer_stride": 1 << 30}, 0, ""),

@@ -82,9 +82,8 @@ class Pair:
         self.ops.attention(stream, self.gpu, layer, q.cuda(), g.cuda() if gate else None, self.ints(start), at, y, rows, width + pad, width + 4, width + 8, nq,
                            max(counts), longest)
         got = y.double().cpu().numpy()
-        pairs = max(counts) * (nq // self.gpu.nkv)
         want, tol = self.model.attention(layer, q[:rows, :width].double().numpy().reshape(rows, nq, hd), g[:rows, :width].double().numpy() if gate else None,
-                                         start, None if qpos is None else np.array(qpos), torch.finfo(act).eps / 2, pairs, act == torch.bfloat16)
+                                         start, None if qpos is None else np.array(qpos), torch.finfo(act).eps / 2, act == torch.bfloat16)
         assert (got[:, width:] == SENTINEL).all() and (got[rows:] == SENTINEL).all(), "written past the rows"
         got = got[:rows, :width]
         assert np.array_equal(np.isnan(got), np.isnan(want)), "NaN where there should be none, or the other way round"
@@ -340,10 +339,20 @@ def test_attention_in_chunks(k, act, lens, counts, hd):
     k.dev.check_status()
 
 
+def test_attention_long_sequences_whole(k):
+    """So many sequences that none is cut: a warp's share of the long ones is more tiles than it remembers pages of at a time."""
+    p = _filled(k, [9000, 4500] + [5] * 90, 1, 128, 32)
+    p.attend([1] * 92, 2)
+    p = _filled(k, [2400] + [7] * 320, 1, 256, 128)
+    p.attend([1] * 321, 9)
+    k.dev.check_status()
+
+
 def test_attention_few_rows_of_many_heads(k, act):
-    """16 heads a kv head: one row fills a tile; 2 rows take two."""
-    p = _filled(k, [70, 300], 2, 128, 32)
-    p.attend([1, 2], 32)
+    """16 heads a kv head: rows whose heads lie in two tiles of pairs."""
+    for hd, counts in ((128, [1, 2]), (128, [1, 5]), (256, [2, 3])):
+        p = _filled(k, [70, 300], 2, hd, 32)
+        p.attend(counts, 32)
     k.dev.check_status()
 
 
