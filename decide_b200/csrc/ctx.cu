@@ -286,6 +286,7 @@ int dc_warm_up(dc_ctx* ctx) {
     if (rc == DC_OK) rc = dc_attention_tc_warm(ctx);
     if (rc == DC_OK) rc = dc_delta_chunk_warm(ctx);
     if (rc == DC_OK) rc = dc_kv8_attention_warm(ctx);
+    if (rc == DC_OK) rc = dc_kv8_attention_tc_warm(ctx);
     return rc;
 }
 

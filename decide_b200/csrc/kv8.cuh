@@ -18,6 +18,7 @@ enum {
 int dc_kv8_require(dc_ctx* ctx, const char* who, const dc_kv8_cache* cache);
 
 int dc_kv8_attention_warm(dc_ctx* ctx);
+int dc_kv8_attention_tc_warm(dc_ctx* ctx);
 
 // Makes the context's device current for the scope of an entry point: the caller's current device may be another one.
 struct dc_device_scope {

@@ -4,9 +4,8 @@
 // s_j = a_j (q . k'_j) hd^-1/2 and o = sum_j softmax(s)_j b_j v'_j. Taking the V scale into the exponent, with t_j = s_j log2(e) + e_v(j):
 //     o = sum_j 2^(t_j - m) v'_j / sum_j 2^(t_j - m) 2^-e_v(j),    m any upper bound of t_j up to a factor,
 // so that one running maximum serves both sums, the weights of the V product are relative to the row's largest TERM, and no code is
-// ever scaled: codes go into the tensor cores as fp16, exactly. The weights are rounded once, to fp16, because the V product takes
-// 16-bit operands (relative to the row's largest term they lose nothing that matters); the total adds them in fp32 before that, since
-// a key whose page has a small V scale may weigh much in it and little in the product.
+// ever scaled: codes go into the tensor cores as fp16, exactly. The V product takes the weights in fp16 (relative to the row's largest
+// term they lose nothing that matters); the total is fp32.
 //
 // K/V bytes bound it when there are few rows. A CTA takes up to 8 NT (query row, head of the group) pairs that share a kv head's codes; its
 // warps take 16 keys each in turn with mma.sync m16n8k16, codes as the A operand (so that 16 keys, or 16 columns of V, fill it, and
@@ -26,7 +25,7 @@
 // Keys are cut into chunks over CTAs; partial results meet in the workspace, and the CTA of a tile that finishes last (a counter tells)
 // joins them in chunk order, so that the result does not depend on timing.
 #include <cmath>
-#include "kv8.cuh"
+#include "kv8_attn.cuh"
 #include "ptx.cuh"
 
 namespace {
@@ -34,9 +33,6 @@ namespace {
 using namespace dc;
 
 constexpr uint32_t kTile = 16;       // keys a warp takes at a time; a page holds a whole number of tiles
-constexpr float kNone = -1e30f;      // running maximum of a row that has seen nothing
-constexpr float kStep = 8.0f;        // the maximum follows only when it grows by more than 2^8
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD, int NT>
 struct Shape {
@@ -55,11 +51,6 @@ struct Shape {
     static constexpr int kBlocks = (HD * NT <= 256 ? 16 : HD * NT <= 384 ? 12 : 8) / kWarps;   // CTAs an SM that registers and shared memory leave room for
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -74,83 +65,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// The two codes in the low (high) 16 bits as fp16, exactly.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(h) : "r"(w));
-    return h;
-}
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(h) : "r"(w));
-    return h;
-}
-
-// The rows of a tile: what the kernel and the join agree on.
-struct Rows {
-    uint32_t start, count, len;   // of the sequence: first packed row, rows, tokens
-    bool ok;
-};
-__device__ __forceinline__ Rows rows_of(const dc_kv8_cache& c, const uint32_t* q_start, uint32_t j, uint32_t rows, uint32_t max_q) {
-    Rows r;
-    r.start = q_start[j];
-    const uint32_t end = q_start[j + 1];
-    r.len = c.lens[j];
-    r.count = end - r.start;
-    r.ok = end >= r.start && end <= rows && r.count <= max_q;
-    return r;
-}
-// Tokens that row i of the sequence attends; *past is set where its position lies at or past the length.
-__device__ __forceinline__ uint32_t visible(const Rows& r, const uint32_t* qpos, uint32_t i, bool* past) {
-    if (!qpos) {
-        const uint32_t behind = r.count - 1 - i;   // rows after this one
-        if (behind >= r.len) {
-            *past = r.len != 0u;
-            return 0u;
-        }
-        return r.len - behind;
-    }
-    const uint32_t p = qpos[r.start + i];
-    if (p == DC_KV8_NO_KEYS || r.len == 0u) return 0u;
-    if (p >= r.len) *past = true;
-    return min(p, r.len - 1) + 1;
-}
-
-struct Args {
-    dc_kv8_cache c;   // k, v and the scales point at the layer
-    const uint16_t* q;
-    const float* gate;
-    const uint32_t* q_start;
-    const uint32_t* qpos;
-    uint16_t* y;
-    float* part;
-    uint32_t* done;   // a counter per tile, zero between launches
-    int* status;
-    uint32_t rows, ldq, ldg, ldy, group, max_q, max_len, tiles, chunk, chunks;
-    float scale;      // hd^-1/2 log2(e)
-};
-
-// Columns d .. d + 7 of a pair: sums over the total, gate, 16 bits. A row that attends nothing has no total: zero.
-template <typename Act>
-__device__ __forceinline__ void finish(const Args& a, const Rows& r, uint32_t pair, uint32_t kvh, uint32_t d, uint32_t hd, float total, float (&o)[8]) {
-    const uint32_t row = r.start + pair / a.group, col = (kvh * a.group + pair % a.group) * hd + d;
-    const float by = total == 0.f ? 0.f : 1.0f / total;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] *= by;
-    if (a.gate) {
-        const float4 g0 = *reinterpret_cast<const float4*>(a.gate + static_cast<size_t>(row) * a.ldg + col);
-        const float4 g1 = *reinterpret_cast<const float4*>(a.gate + static_cast<size_t>(row) * a.ldg + col + 4);
-        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] *= sigmoid_f(g[i]);
-    }
-    *reinterpret_cast<uint4*>(a.y + static_cast<size_t>(row) * a.ldy + col) =
-        make_uint4(Act::pack(o[0], o[1]), Act::pack(o[2], o[3]), Act::pack(o[4], o[5]), Act::pack(o[6], o[7]));
-}
-
 // One CTA: 8 NT (row, head) pairs of a sequence's kv head over one chunk of its keys.
 template <typename Act, int HD, int NT>
-__global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlocks) kv8_attn_kernel(const Args a) {
+__global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlocks) kv8_attn_kernel(const Kv8Args a) {
     using S = Shape<HD, NT>;
     constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
     constexpr int kKVec = HD / 64;         // vectors of a key a lane holds
@@ -174,9 +91,9 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     // is not known yet, the table is read ahead of it (never past its row).
     const uint32_t key0 = z * a.chunk;
     const uint32_t* table = a.c.table + static_cast<size_t>(j) * a.c.max_pages;
-    auto column = [&](uint32_t i) { return (key0 + (warp + kWarps * i) * kTile) / a.c.page_size; };
+    auto column = [&](uint32_t i) { return (key0 + (warp + kWarps * i) * kTile) >> a.page_shift; };
     uint32_t page_ahead = column(lane) < a.c.max_pages ? table[column(lane)] : 0u;
-    const Rows r = rows_of(a.c, a.q_start, j, a.rows, a.max_q);
+    const Kv8Rows r = kv8_rows(a.c, a.q_start, j, a.rows, a.max_q);
     const bool reports = kvh == 0 && z == 0 && threadIdx.x == 0;
     if (!r.ok) {
         if (reports && mt == 0) kv8_flag(a.status, DC_STATUS_KV8_OFFSETS);
@@ -192,7 +109,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     const bool on = lane < static_cast<int>(kPairs) && pair0 + lane < pairs;
     {
         bool past = false;
-        if (on) n = visible(r, a.qpos, (pair0 + lane) / a.group, &past);
+        if (on) n = kv8_visible(r, a.qpos, kv8_row_of(a, pair0 + lane), &past);
         if (past && kvh == 0 && z == 0 && warp == 0) kv8_flag(a.status, DC_STATUS_KV8_POSITION);
     }
     const uint32_t most = __reduce_max_sync(0xffffffffu, n), least = __reduce_min_sync(0xffffffffu, on ? n : 0xffffffffu);
@@ -213,7 +130,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                 kv8_flag(a.status, DC_STATUS_KV8_PAGE);
                 page = 0;
             }
-            page_at = page * a.c.page_stride + kvh * a.c.head_stride + (key % a.c.page_size) * a.c.token_stride;
+            page_at = page * a.c.page_stride + kvh * a.c.head_stride + (key & (a.c.page_size - 1)) * a.c.token_stride;
             next_k = a.c.k_scale[static_cast<size_t>(page) * a.c.nkv + kvh];
             next_v = a.c.v_scale[static_cast<size_t>(page) * a.c.nkv + kvh];
             if (!inside) next_k = __uint_as_float(0x7fffffffu);   // what attends it is NaN
@@ -246,35 +163,16 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     }
 
     // q as B fragments, in the order that the K codes lie in: k-step 4 v + w of lane (g, t) takes hd 64 v + 16 t + 4 w + {0, 1 | 2, 3}, 8 bytes
-    // of q as they are. A bf16 row is first divided by a power of two that brings its largest magnitude to [2^14, 2^15): then its 8
-    // bits fit fp16 but for elements 2^-28 below it. fp16 rows go in as they are.
+    // of q as they are.
     for (uint32_t p = warp; p < kPairs; p += kWarps) {
         const bool there = pair0 + p < pairs;
-        const uint32_t row = r.start + (pair0 + p) / a.group, h = kvh * a.group + (pair0 + p) % a.group;
+        const uint32_t of = kv8_row_of(a, pair0 + p), row = r.start + of, h = kvh * a.group + pair0 + p - of * a.group;
         const uint16_t* src = a.q + static_cast<size_t>(row) * a.ldq + static_cast<size_t>(h) * HD;
         constexpr int kWords = HD / 128;   // 8-byte pieces a lane holds: piece lane + 32 i is hd 4 (lane + 32 i) ..
         uint2 x[kWords];
 #pragma unroll
         for (int i = 0; i < kWords; ++i) x[i] = there ? *reinterpret_cast<const uint2*>(src + 4 * (lane + 32 * i)) : make_uint2(0, 0);
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) top = __vmaxu2(top, __vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu));
-        top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-        float up = 1.f;
-        if (Act::kUmmaFormat == 1) {
-            const uint32_t e = top >> 7;   // exponent field of the largest
-            // 2^(e - 127) -> 2^14; fields beyond 1 .. 254 (zeros, subnormals, infinities) take the nearest
-            const int shift = min(max(static_cast<int>(e), 1), 254) - 127 - 14;
-            const int half = shift / 2;   // two factors: 2^-shift alone may pass fp32's exponents
-            const float down = kv8_exp2i(-half), rest_down = kv8_exp2i(-(shift - half));
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                x[i].x = ActF16::pack(Act::lo(x[i].x) * down * rest_down, Act::hi(x[i].x) * down * rest_down);
-                x[i].y = ActF16::pack(Act::lo(x[i].y) * down * rest_down, Act::hi(x[i].y) * down * rest_down);
-            }
-            up = kv8_exp2i(half) * kv8_exp2i(shift - half);
-        }
-        if (!(Act::one(static_cast<uint16_t>(top)) <= 3.4028235e38f)) up = __uint_as_float(0x7fffffffu);   // a row that is not finite: NaN
+        const float up = kv8_query_row<Act, kWords>(x, kv8_query_top<kWords>(x));
         if (lane == 0) rank[p] = up;
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
@@ -291,7 +189,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             mul[b][e] = a.scale * rank[8 * b + 2 * t + e];
-            m[b][e] = kNone;
+            m[b][e] = kKv8None;
             l[b][e] = 0.f;
         }
     constexpr bool kKeepQ = NT * HD <= 128;   // q fragments in registers where there is room
@@ -359,7 +257,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
 #pragma unroll
         for (int b = 0; b < NT; ++b)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[b][e], s[b][2 + e]) > m[b][e] + kStep;
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[b][e], s[b][2 + e]) > m[b][e] + kKv8Step;
         if (__any_sync(0xffffffffu, grow)) {
             // the eight lanes of a pair agree on the new maximum; pairs whose maximum stays put scale by 1
 #pragma unroll
@@ -380,14 +278,25 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                     }
                 }
         }
-        uint32_t p0[NT], p1[NT];   // B fragments of the weights
+        // The weights as B fragments. One set of eight pairs goes in twice, rounded to fp16 and what that left (22 bits for eight more MMAs
+        // that memory hides); two sets go in once, and the total adds them as they go in (kv8_total).
+        constexpr bool kTwice = NT == 1;
+        uint32_t p0[NT], p1[NT], q0 = 0, q1 = 0;
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             const float w00 = ex2(s[b][0] - m[b][0]), w01 = ex2(s[b][1] - m[b][1]), w10 = ex2(s[b][2] - m[b][0]), w11 = ex2(s[b][3] - m[b][1]);
-            l[b][0] = fmaf(w00 + w10, back, l[b][0]);
-            l[b][1] = fmaf(w01 + w11, back, l[b][1]);
-            p0[b] = transpose8(ActF16::pack(w00, w01));
-            p1[b] = transpose8(ActF16::pack(w10, w11));
+            const uint32_t lo = ActF16::pack(w00, w01), hi = ActF16::pack(w10, w11);
+            if (kTwice) {
+                l[b][0] = fmaf(w00 + w10, back, l[b][0]);
+                l[b][1] = fmaf(w01 + w11, back, l[b][1]);
+                q0 = transpose8(ActF16::pack(w00 - ActF16::lo(lo), w01 - ActF16::hi(lo)));
+                q1 = transpose8(ActF16::pack(w10 - ActF16::lo(hi), w11 - ActF16::hi(hi)));
+            } else {
+                l[b][0] = fmaf(kv8_total(w00, ActF16::lo(lo)) + kv8_total(w10, ActF16::lo(hi)), back, l[b][0]);
+                l[b][1] = fmaf(kv8_total(w01, ActF16::hi(lo)) + kv8_total(w11, ActF16::hi(hi)), back, l[b][1]);
+            }
+            p0[b] = transpose8(lo);
+            p1[b] = transpose8(hi);
         }
 #pragma unroll
         for (int v = 0; v < kVVec; ++v) {
@@ -409,6 +318,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                 const uint32_t a0 = low_codes(w0), a1 = high_codes(w0), a2 = low_codes(w1), a3 = high_codes(w1);
 #pragma unroll
                 for (int b = 0; b < NT; ++b) mma_f16(o[b][8 * v + d], a0, a1, a2, a3, p0[b], p1[b]);
+                if (kTwice) mma_f16(o[0][8 * v + d], a0, a1, a2, a3, q0, q1);
             }
         }
         const uint32_t next = stage == 0 ? S::kStages - 1 : stage - 1;   // (i + kStages - 1) % kStages
@@ -445,7 +355,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     const uint32_t here = min(kPairs, pairs - pair0);
     for (uint32_t e = threadIdx.x; e < here * (HD / 8); e += kThreads) {
         const uint32_t p = e / (HD / 8), d = e % (HD / 8) * 8;
-        float top = kNone, total = 0.f, x[8] = {};
+        float top = kKv8None, total = 0.f, x[8] = {};
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, all[(w * kPairs + p) * S::kLd + HD]);
 #pragma unroll
@@ -457,7 +367,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
             for (int i = 0; i < 8; ++i) x[i] = fmaf(from[d + i], by, x[i]);
         }
         if (whole) {
-            finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
+            kv8_finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
         } else {
             float* to = parts + (z * kPairs + p) * S::kLd;
             *reinterpret_cast<float4*>(to + d) = make_float4(x[0], x[1], x[2], x[3]);
@@ -484,7 +394,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     for (uint32_t e = groups == 1 ? threadIdx.x : threadIdx.x % items; e < items && group < groups; e += kThreads) {
         const uint32_t p = e / kCols, d = e % kCols * 8;
         const float* from = parts + p * S::kLd;
-        float top = kNone, total = 0.f, x[8] = {};
+        float top = kKv8None, total = 0.f, x[8] = {};
         for (uint32_t k0 = group; k0 < chunks; k0 += 4 * groups) {   // four chunks' loads in flight
             float2 ml[4];
             float4 u[4], w[4];
@@ -495,7 +405,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                 ml[i] = __ldcg(reinterpret_cast<const float2*>(at + HD));
                 u[i] = __ldcg(reinterpret_cast<const float4*>(at + d));
                 w[i] = __ldcg(reinterpret_cast<const float4*>(at + d + 4));
-                if (k >= chunks) ml[i] = make_float2(kNone, 0.f), u[i] = w[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k >= chunks) ml[i] = make_float2(kKv8None, 0.f), u[i] = w[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             const float now = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), old = ex2(top - now);
             top = now;
@@ -511,7 +421,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
             }
         }
         if (groups == 1) {
-            finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
+            kv8_finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
         } else {
             float* to = sums + (group * here + p) * S::kLd;
             *reinterpret_cast<float4*>(to + d) = make_float4(x[0], x[1], x[2], x[3]);
@@ -523,7 +433,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     __syncthreads();
     if (threadIdx.x < items) {
         const uint32_t p = threadIdx.x / kCols, d = threadIdx.x % kCols * 8;
-        float top = kNone, total = 0.f, x[8] = {};
+        float top = kKv8None, total = 0.f, x[8] = {};
         for (uint32_t k = 0; k < groups; ++k) top = fmaxf(top, sums[(k * here + p) * S::kLd + HD]);
         for (uint32_t k = 0; k < groups; ++k) {
             const float* at = sums + (k * here + p) * S::kLd;
@@ -532,11 +442,11 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(at[d + i], by, x[i]);
         }
-        finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
+        kv8_finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
     }
 }
 
-typedef void (*attn_fn)(const Args);
+typedef void (*attn_fn)(const Kv8Args);
 struct Variant {
     attn_fn f;
     int bytes, threads, blocks;
@@ -551,18 +461,13 @@ Variant pick(uint32_t hd, uint32_t nt) {
 
 // How a call is cut: tiles of 8 nt (row, head) pairs, chunks of `chunk` keys.
 constexpr uint64_t kDoneCounters = DC_KV8_DONE_COUNTERS;
-struct Cut {
-    uint32_t nt, tiles, max_len, chunk, chunks;
-    uint64_t ctas;
-};
-Cut cut_of(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
-    Cut t;
+Kv8Cut cut_of(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
+    Kv8Cut t;
     // Pairs in eights, a CTA each: many narrow tiles hide their latencies better than few wide ones (24 pairs over 2,307 keys: 10.0 us in
     // eights, 12.1 in sixteens), until the tiles alone are more than the GPU holds at once; then two eights share a pass over the codes
     // (16 pairs of 64 x 1,200 keys: 44 against 52 us).
     const uint64_t eights = (static_cast<uint64_t>(max_q) * (nq / c->nkv) + 7) / 8;
-    const uint32_t cap = c->max_pages * c->page_size;
-    const uint32_t len = max_len == 0 || max_len > cap ? cap : max_len;
+    const uint32_t len = max_len;
     const uint64_t items = static_cast<uint64_t>(c->n_seqs) * c->nkv;
     Variant v = pick<dc::ActF16>(c->hd, 1);
     t.nt = eights > 1 && items * eights > static_cast<uint64_t>(ctx->sm_count) * v.blocks ? 2 : 1;
@@ -580,14 +485,23 @@ Cut cut_of(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q
         if (parts > room) parts = room < 1 ? 1 : room;
     }
     t.chunk = static_cast<uint32_t>(((len + parts - 1) / parts + step - 1) / step * step);
-    t.max_len = len;
     t.chunks = (len + t.chunk - 1) / t.chunk;
     t.ctas = whole * t.chunks;
+    t.part_bytes = t.chunks > 1 ? t.ctas * 8 * t.nt * (c->hd + 4) * sizeof(float) : 0;
     return t;
 }
-size_t part_bytes(const dc_kv8_cache* c, const Cut& t) {
-    if (t.chunks <= 1) return 0;
-    return static_cast<size_t>(t.ctas) * 8 * t.nt * (c->hd + 4) * sizeof(float);
+
+// The longest sequence that a call may meet.
+uint32_t longest(const dc_kv8_cache* c, uint32_t max_len) {
+    const uint32_t cap = c->max_pages * c->page_size;
+    return max_len == 0 || max_len > cap ? cap : max_len;
+}
+
+// Whole tiles of the tensor cores (256 pairs a CTA) against eights: 128 pairs and more of a sequence, half that over long ones. Measured, us,
+// tcgen05 and here: 64 pairs over 2,307 keys 18 and 13, over 16,000 keys 32 and 46; 64 sequences of 64 pairs over 1,200 keys 171
+// and 132; 256 pairs over 2,307 keys 24 and 24, over 16,000 keys 42 and 124; 16 sequences of 256 pairs over 1,500 keys 64 and 150.
+bool on_tcgen05(const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
+    return c->hd == 128 && static_cast<uint64_t>(max_q) * (nq / c->nkv) >= (max_len < 8192 ? 128 : 64);
 }
 
 }  // namespace
@@ -607,7 +521,8 @@ int dc_kv8_attention_warm(dc_ctx* ctx) {
 
 extern "C" size_t dc_kv8_attention_scratch_bytes(dc_ctx* ctx, const dc_kv8_cache* cache, uint32_t nq, uint32_t max_q, uint32_t max_len) {
     if (!ctx || dc_kv8_check(cache, nullptr, 0) != DC_OK || nq == 0 || nq % cache->nkv || max_q == 0) return 0;
-    return part_bytes(cache, cut_of(ctx, cache, nq, max_q, max_len));
+    const uint32_t len = longest(cache, max_len);
+    return (on_tcgen05(cache, nq, max_q, len) ? dc_kv8_attention_tc_cut(ctx, cache, nq, max_q, len) : cut_of(ctx, cache, nq, max_q, len)).part_bytes;
 }
 
 extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t layer, const void* q, const float* gate,
@@ -628,10 +543,14 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     DC_REQUIRE(ctx, reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0, "kv8_attention: q and y must be 16-byte aligned");
     if (rows == 0 || max_q == 0) return DC_OK;   // no rows: nothing to write
     const uint32_t most = max_q < rows ? max_q : rows;
+    if (static_cast<uint64_t>(most) * (nq / cache->nkv) >= (1ull << 28))
+        return dc_fail(ctx, DC_UNSUPPORTED, "kv8_attention: %u rows of %u heads per kv head in one sequence (below 2^28 together)", most, nq / cache->nkv);
     const dc_device_scope scope(ctx);
-    const Cut t = cut_of(ctx, cache, nq, most, max_len);
+    const uint32_t len = longest(cache, max_len);
+    const bool tc = on_tcgen05(cache, nq, most, len);
+    const Kv8Cut t = tc ? dc_kv8_attention_tc_cut(ctx, cache, nq, most, len) : cut_of(ctx, cache, nq, most, len);
     DC_REQUIRE(ctx, t.ctas < 0x7fffffffull, "kv8_attention: %llu CTAs: fewer rows or sequences a call", static_cast<unsigned long long>(t.ctas));
-    Args a;
+    Kv8Args a;
     a.c = *cache;
     a.c.k = static_cast<uint8_t*>(cache->k) + layer * cache->layer_stride;
     a.c.v = static_cast<uint8_t*>(cache->v) + layer * cache->layer_stride;
@@ -641,7 +560,7 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     a.done = ctx->kv8_done;
     if (t.chunks > 1) {
         void* ws = nullptr;
-        if ((rc = dc_get_workspace(ctx, part_bytes(cache, t), "kv8_attention", &ws)) != DC_OK) return rc;
+        if ((rc = dc_get_workspace(ctx, t.part_bytes, "kv8_attention", &ws)) != DC_OK) return rc;
         a.part = static_cast<float*>(ws);
     }
     if ((rc = dc_kv8_attention_warm(ctx)) != DC_OK) return rc;
@@ -651,11 +570,13 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     a.qpos = qpos;
     a.y = static_cast<uint16_t*>(y);
     a.status = ctx->status_dev;
-    a.rows = rows, a.ldq = ldq, a.ldg = ldg, a.ldy = ldy, a.group = nq / cache->nkv, a.max_q = most, a.max_len = t.max_len;
+    a.rows = rows, a.ldq = ldq, a.ldg = ldg, a.ldy = ldy, a.group = nq / cache->nkv, a.max_q = most, a.max_len = len;
     a.tiles = t.tiles, a.chunk = t.chunk, a.chunks = t.chunks;
-    a.scale = kLog2e / sqrtf(static_cast<float>(cache->hd));
+    a.page_shift = __builtin_ctz(cache->page_size), a.group_inverse = a.group > 1 ? static_cast<uint32_t>((1ull << 32) / a.group + 1) : 0u;
+    a.scale = kKv8Log2e / sqrtf(static_cast<float>(cache->hd));
     const bool f16 = ctx->act_dtype == DC_ACT_F16;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (tc) return dc_kv8_attention_tc(ctx, s, a, t.ctas);
     const Variant v = f16 ? pick<dc::ActF16>(cache->hd, t.nt) : pick<dc::ActBF16>(cache->hd, t.nt);
     v.f<<<static_cast<uint32_t>(t.ctas), v.threads, v.bytes, s>>>(a);
     return dc_check_launch(ctx, "kv8_attention");

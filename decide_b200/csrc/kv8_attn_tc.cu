@@ -1,0 +1,629 @@
+// dc_kv8_attention for many rows a sequence (heads of 128): the mathematics of kv8_attn.cu on tcgen05.
+//
+// Products bound it: 4 * 128 operations for each (pair, key), a pair being a (query row, head of the group), against one exponential
+// and one weight to round. A CTA takes 256 pairs that share a kv head as two tiles of 128, the lanes of tensor memory, which pass the
+// tensor cores back and forth: while one tile's scores are turned into weights, the other's products run.
+//   warps 9..11   codes -> fp16 K and V tiles of 128 keys in shared memory, two stages each. Both lie as rows of keys, 64 columns (128 bytes)
+//                 to a swizzled block: K is read as the K-major operand of S = Q K^T, V as the MN-major operand of O += P V, so V needs
+//                 no transposition. The 256 pairs share this work.
+//   warp 8        issues S = Q K^T and O += P V of the two tiles in turn, 64 keys at a time. A tile has two buffers of scores:
+//                 while one is turned into weights the other fills, so that neither side waits for the other's round trip (with one
+//                 buffer of 128 keys a step took 4,400 cycles, 1,750 of them between the last weight and the next scores)
+//   warps 0..3, 4..7  softmax of a tile, one thread per pair: 64 scores into registers, their maximum, then the weights, which go back
+//                 into the columns that the scores came from as the A operand of the V product. Page scales are applied per 16 keys, to
+//                 the maximum of a group and inside the exponential's argument: no instruction per score.
+// Warp 8 shares its scheduler with two softmax warps and nothing else: with a filler there too its issue of products was the bound.
+// The running maximum is lazy as in kv8_attn.cu: O in tensor memory is rescaled only when it grows by more than 2^8.
+// Tensor memory: 2 x (2 x 64 columns of scores + 128 of O). Shared memory: q 64 KB, K and V 64 KB each: one CTA an SM.
+// Where there are fewer tiles than SMs the keys are cut into chunks, whose results a second kernel joins in chunk order.
+// Every wait is bounded; when one gives up the CTA raises the status word, waits for its products in flight and returns.
+#include "kv8_attn.cuh"
+#include "ptx.cuh"
+
+namespace {
+
+using namespace dc;
+
+constexpr int HD = 128;
+constexpr int kPairs = 256;
+constexpr uint32_t kKeys = 128;      // keys a stage of K or V holds
+constexpr uint32_t kHalf = 64;       // keys a product of scores covers
+constexpr int kThreads = 384;
+constexpr int kFillers = 3;          // warps that turn codes into tiles
+constexpr int kUnits = 11;           // of 32 units of four keys a stage, the first two fillers take 11 each and the last 10
+constexpr uint32_t kTmemCols = 512;
+constexpr int kLd = HD + 4;          // floats of a pair's partial result
+constexpr int kScaleSlots = 4;
+
+struct Smem {
+    static constexpr uint32_t kAtom = 128 * 128;            // [128 rows][64 x 16 bit]
+    static constexpr uint32_t kQ = 0;                       // [2 tiles][2 halves of hd]
+    static constexpr uint32_t kK = kQ + 4 * kAtom;          // [2 stages][2 halves]
+    static constexpr uint32_t kV = kK + 4 * kAtom;
+    static constexpr uint32_t kScales = kV + 4 * kAtom;     // float4 [kScaleSlots][8], of 16 keys: K scale, log2 of the V scale, 1 / V scale
+    static constexpr uint32_t kRank = kScales + kScaleSlots * 8 * 16;   // float [256]
+    static constexpr uint32_t kSeen = kRank + kPairs * 4;   // u32 [256]
+    static constexpr uint32_t kBars = kSeen + kPairs * 4;
+    static constexpr uint32_t kBytes = kBars + 32 * 8;
+};
+
+__device__ __forceinline__ void sts16(uint32_t to, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// Advances a two-stage ring.
+struct Ring {
+    uint32_t stage = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        stage ^= 1u;
+        if (stage == 0) phase ^= 1u;
+    }
+};
+
+// V's descriptor: MN-major, 128-byte swizzle. Keys are rows of 128 bytes in groups of 8 (1024 bytes); the two halves of hd lie an atom apart.
+__device__ __forceinline__ uint64_t desc_mn128(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(Smem::kAtom >> 4) << 16;   // leading byte offset: from 64 columns to the next 64
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;          // stride byte offset: from 8 keys to the next 8
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+// 64 keys of a warp's 32 pairs: scores out of tensor memory, their maximum, then the weights into the columns that the scores came from.
+// MASKED: some pair of the warp does not see all 64 keys; `vis` of them it does. settled(): O may be rescaled.
+template <bool MASKED, typename F>
+__device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, const float4* sc, float mul, int vis, bool scale_o, float& m, float& l, F settled) {
+    uint32_t s[2][32];
+    tmem_ld_32x32(col_s, s[0]);
+    tmem_ld_32x32(col_s + 32, s[1]);
+    tmem_ld_wait();
+    float top = kKv8None;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        uint32_t* v = s[g >> 1] + 16 * (g & 1);
+        float t[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            if (MASKED) {
+                v[e] = 16 * g + e < vis ? v[e] : 0xff800000u;   // out of the maximum
+                v[e + 1] = 16 * g + e + 1 < vis ? v[e + 1] : 0xff800000u;
+            }
+            t[(e >> 1) & 1] = fmaxf(fmaxf(t[(e >> 1) & 1], __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+        }
+        const float2 ab = *reinterpret_cast<const float2*>(sc + g);
+        top = fmaxf(top, fmaf(fmaxf(t[0], t[1]), mul * ab.x, ab.y));
+    }
+    const bool grow = top > m + kKv8Step;
+    if (__any_sync(0xffffffffu, grow)) {
+        // O and the total follow the new maximum (pairs whose maximum stays put scale by 1)
+        const float by = grow ? ex2(m - top) : 1.0f;
+        l *= by;
+        if (grow) m = top;
+        if (scale_o) {
+            if (!settled()) return false;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint32_t v[16];
+                tmem_ld_32x32_x16(col_o + 16 * c, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * by);
+                tmem_st_32x32_x16(col_o + 16 * c, v);
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t w[16];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const uint32_t* v = s[h] + 16 * g;
+            const float4 ab = sc[2 * h + g];
+            const float by = mul * ab.x, off = ab.y - m;
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                float p0 = ex2(fmaf(__uint_as_float(v[e]), by, off)), p1 = ex2(fmaf(__uint_as_float(v[e + 1]), by, off));
+                if (MASKED) {   // explicitly: a scale that is NaN, or a multiplier of zero, makes no zero of -infinity
+                    p0 = 32 * h + 16 * g + e < vis ? p0 : 0.f;
+                    p1 = 32 * h + 16 * g + e + 1 < vis ? p1 : 0.f;
+                }
+                w[8 * g + e / 2] = ActF16::pack(p0, p1);
+                sum0 += p0;   // (the total of the rounded weights, as kv8_attn.cu takes it, costs three instructions a weight: 300 -> 357 us
+                sum1 += p1;   // for 2,048 rows over 8,191 keys, and brings the error from 1.3 to 1.2 times that of rounding the output)
+            }
+            l = fmaf(sum0 + sum1, ab.z, l);
+        }
+        tmem_st_32x32_x16(col_s + 16 * h, w);
+    }
+    return true;
+}
+
+template <typename Act>
+__global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args a) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
+    uint64_t* k_full = bars;            // [2] the fillers have written K
+    uint64_t* v_full = bars + 2;        // [2]
+    uint64_t* k_free = bars + 4;        // [2] both tiles' score products are done
+    uint64_t* v_free = bars + 6;        // [2]
+    uint64_t* s_full = bars + 8;        // [2 tiles][2 buffers] scores are there
+    uint64_t* p_full = bars + 12;       // [2][2] the tile's four warps have written the weights (and rescaled O)
+    uint64_t* pv_done = bars + 16;      // [2] a V product of the tile, and every product before it, is done
+    uint64_t* scale_full = bars + 18;   // [kScaleSlots]
+    uint64_t* q_full = bars + 22;       // warps 0..7 have written q
+    uint64_t* drain_bar = bars + 23;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    volatile uint32_t* never_flag = tmem_slot + 2;
+    float4* scales = reinterpret_cast<float4*>(smem + Smem::kScales);
+    float* rank = reinterpret_cast<float*>(smem + Smem::kRank);
+    uint32_t* seen = reinterpret_cast<uint32_t*>(smem + Smem::kSeen);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t id = blockIdx.x;
+    const uint32_t z = id % a.chunks;
+    id /= a.chunks;
+    const uint32_t tile_id = id, kvh = id % a.c.nkv;
+    id /= a.c.nkv;
+    const uint32_t mt = a.tiles - 1 - id % a.tiles, j = id / a.tiles;   // the last rows, which see the most keys, first
+
+    const Kv8Rows r = kv8_rows(a.c, a.q_start, j, a.rows, a.max_q);
+    const bool reports = kvh == 0 && z == 0;
+    if (!r.ok) {
+        if (reports && tid == 0) kv8_flag(a.status, DC_STATUS_KV8_OFFSETS);
+        return;
+    }
+    const uint32_t pair0 = mt * kPairs, pairs = r.count * a.group;
+    if (pair0 >= pairs) return;
+    if (r.len > a.max_len) {
+        if (reports && tid == 0) kv8_flag(a.status, DC_STATUS_KV8_LENGTH);
+        return;
+    }
+    const uint32_t here = min(static_cast<uint32_t>(kPairs), pairs - pair0);
+    const bool two = here > 128;   // the second tile has rows
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], kFillers);
+            mbar_init(&v_full[i], kFillers);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_free[i], 1);
+            mbar_init(&pv_done[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+        }
+        for (int i = 0; i < kScaleSlots; ++i) mbar_init(&scale_full[i], 1);
+        mbar_init(q_full, two ? 8 : 4);
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0u;
+        *never_flag = 0u;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    // tokens that the pairs attend, and the most that any of them does: every warp for itself, so that none waits for another
+    uint32_t most = 0;
+    {
+        bool past = false;
+#pragma unroll
+        for (int i = 0; i < kPairs / 32; ++i) {
+            const uint32_t p = 32 * i + lane, n = p < here ? kv8_visible(r, a.qpos, kv8_row_of(a, pair0 + p), &past) : 0u;
+            if (warp == i) seen[p] = n;
+            most = max(most, n);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (past && reports && warp == 0) kv8_flag(a.status, DC_STATUS_KV8_POSITION);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t key0 = z * a.chunk;
+    const bool whole = most <= a.chunk;
+    const bool idle = z && key0 >= most;             // nothing of this tile in this chunk
+    const uint32_t key1 = min(most, key0 + a.chunk);
+    const uint32_t halves = idle ? 0u : (key1 - key0 + kHalf - 1) / kHalf, steps = (halves + 1) / 2;
+    const uint32_t tmem = *tmem_slot;                // 0: all of it is ours
+    constexpr uint32_t kColO = 256;                  // S of tile X, buffer B in columns 128 X + 64 B .., O in 256 + 128 X ..
+
+    if (warp > 8) {
+        // -------------------------------------------------------------------------------- codes -> fp16 tiles
+        const int w = warp - 9, unit0 = w * kUnits, units = w == kFillers - 1 ? 32 - unit0 : kUnits;   // units of four keys
+        const uint32_t token = static_cast<uint32_t>(a.c.token_stride), four = 4 * token;
+        const uint32_t* table = a.c.table + static_cast<size_t>(j) * a.c.max_pages;
+        // A lane's place in a unit of four rows of 128 codes: row bits from lane bits 2 and 4, 16-code piece c from bits 0, 1 and 3, so that the
+        // eight lanes of a store's phase, four pieces of two rows, meet all 32 banks of the swizzled tile.
+        const uint32_t fr = ((lane >> 2) & 1) | ((lane >> 4) << 1), c = (lane & 3) | ((lane >> 1) & 4);
+        const uint8_t* kc = static_cast<const uint8_t*>(a.c.k) + kvh * a.c.head_stride + fr * token + 16 * c;
+        const int64_t to_v = static_cast<const uint8_t*>(a.c.v) - static_cast<const uint8_t*>(a.c.k);
+        // The filler's units lie in up to kGroups groups of 16 keys, whose pages every lane looks up for itself, a step ahead of the codes.
+        constexpr int kGroups = 4;
+        const uint32_t group0 = unit0 >> 2;
+        uint32_t page[kGroups];
+        auto look_up = [&](uint32_t step) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const uint32_t key = key0 + step * kKeys + 16 * (group0 + g);
+                page[g] = key < key1 && group0 + g < 8 ? __ldg(table + (key >> a.page_shift)) : 0u;
+            }
+        };
+        const uint8_t* at[kGroups];   // first code of the group in K, this lane's; V lies at the same distance from its first
+        auto to_page = [&](uint32_t step) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const uint32_t key = key0 + step * kKeys + 16 * (group0 + g);
+                if (page[g] >= a.c.n_pages) {
+                    kv8_flag(a.status, DC_STATUS_KV8_PAGE);
+                    page[g] = 0;
+                }
+                at[g] = kc + page[g] * a.c.page_stride + (key & (a.c.page_size - 1)) * token;
+            }
+        };
+        uint4 kx[kUnits], vx[kUnits];
+        auto load = [&](uint4 (&x)[kUnits], int64_t from, uint32_t step) {   // rows 4 (unit0 + i) + fr; zeros past the last token
+            const uint32_t first = key0 + step * kKeys + 4 * unit0 + fr;
+            const bool inside = key0 + (step + 1) * kKeys <= key1;
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                if (i == kUnits - 1 && units < kUnits) break;
+                const uint32_t u = (unit0 & 3) + i;   // from the start of the first group
+                const uint8_t* group = u < 4 ? at[0] : u < 8 ? at[1] : u < 12 ? at[2] : at[3];
+                if (inside || first + 4 * i < key1) x[i] = __ldg(reinterpret_cast<const uint4*>(group + from + (u & 3) * four));
+                else x[i] = make_uint4(0, 0, 0, 0);
+            }
+        };
+        // filler 0 also keeps the scales of the stage's eight groups, lane g those of group g
+        uint32_t scale_page = 0;
+        float k_scale = 0.f, v_scale = 1.f;
+        auto scale_look_up = [&](uint32_t step) {
+            const uint32_t key = key0 + step * kKeys + 16 * (lane & 7);
+            scale_page = key < key1 ? __ldg(table + (key >> a.page_shift)) : 0u;
+        };
+        auto scale_load = [&] {
+            const size_t s = static_cast<size_t>(scale_page < a.c.n_pages ? scale_page : 0u) * a.c.nkv + kvh;
+            k_scale = a.c.k_scale[s];
+            v_scale = a.c.v_scale[s];
+            if (scale_page >= a.c.n_pages) k_scale = __uint_as_float(0x7fffffffu);   // what attends it is NaN
+        };
+        // 16 codes become the 16-byte pieces 2 c and 2 c + 1 of half c / 4 of the row, at piece ^ (row % 8): with row = 4 u + fr that is one
+        // address, its neighbour at ^ 16, and both at ^ 64 for odd u
+        const uint32_t to0 = (smem_u32(smem) + (c >> 2) * Smem::kAtom + (4 * unit0 + fr) * 128 + (((2 * c) ^ fr) & 7) * 16) ^ ((unit0 & 1) * 64);
+        auto store = [&](const uint4 (&x)[kUnits], uint32_t tile) {
+            const uint32_t to = to0 + tile, next = to ^ 64;
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                if (i == kUnits - 1 && units < kUnits) break;
+                sts16((i & 1 ? next : to) + 512 * i, low_codes(x[i].x), high_codes(x[i].x), low_codes(x[i].y), high_codes(x[i].y));
+                sts16((i & 1 ? next ^ 16 : to ^ 16) + 512 * i, low_codes(x[i].z), high_codes(x[i].z), low_codes(x[i].w), high_codes(x[i].w));
+            }
+        };
+        Ring ring;
+        if (steps) {
+            look_up(0);
+            if (w == 0) scale_look_up(0);
+            to_page(0);
+            load(kx, 0, 0);
+            load(vx, to_v, 0);
+            if (w == 0) {
+                scale_load();
+                scale_look_up(1);
+            }
+            look_up(1);
+        }
+        for (uint32_t i = 0; i < steps; ++i) {
+            if (i >= 2 && !mbar_wait(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81)) break;
+            if (w == 0 && lane < 8) {
+                const float e = kv8_log2i(v_scale);   // a NaN reaches the total through the weights, not through 1 / V scale
+                scales[(i % kScaleSlots) * 8 + lane] = make_float4(k_scale, e, isnan(e) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(e)))), 0.f);
+            }
+            store(kx, Smem::kK + ring.stage * 2 * Smem::kAtom);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (w == 0) mbar_arrive(&scale_full[i % kScaleSlots]);
+                mbar_arrive(&k_full[ring.stage]);
+            }
+            const bool more = i + 1 < steps;
+            if (more) {
+                to_page(i + 1);
+                load(kx, 0, i + 1);
+            }
+            if (i >= 2 && !mbar_wait(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82)) break;
+            store(vx, Smem::kV + ring.stage * 2 * Smem::kAtom);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[ring.stage]);
+            if (more) {
+                load(vx, to_v, i + 1);
+                if (w == 0) {
+                    scale_load();
+                    scale_look_up(i + 2);
+                }
+                look_up(i + 2);
+            }
+            ring.next();
+        }
+    } else if (warp == 8) {
+        // -------------------------------------------------------------------------------- products
+        // The whole warp walks the steps and one elected lane issues. Operands of an MMA come from uniform registers: four halves are unrolled,
+        // so that every address is a constant (shared memory starts at a constant, and who owns all of tensor memory starts at column 0).
+        // With addresses worked out at run time an MMA took 60 to 70 cycles to issue, more than it takes to run.
+        if (steps) {
+            constexpr uint32_t idesc_s = umma_idesc(0, 0, 128, kHalf), idesc_o = umma_idesc(0, 0, 128, HD) | (1u << 16);   // B of the V product is MN-major
+            constexpr uint64_t kAtomStep = Smem::kAtom >> 4, kHalfStep = kHalf * 128 >> 4;   // 64 keys: 64 rows of 128 bytes
+            const uint64_t dq = umma_desc_k128(smem_u32(smem) + Smem::kQ), dk = umma_desc_k128(smem_u32(smem) + Smem::kK), dv = desc_mn128(smem_u32(smem) + Smem::kV);
+            const uint32_t n = halves;
+            const bool both = two;
+            auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+                const bool done = mbar_wait(bar, parity, abort_flag, a.status, code);
+                return __all_sync(0xffffffffu, done);
+            };
+            // half u of a round of four: stage u / 2, buffer u % 2; `last`: the stage's last product of the kind
+            auto scores = [&](int x, int u, bool last) {
+                if (elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint64_t off = (ks >> 2) * kAtomStep + 2 * (ks & 3);
+                        const uint64_t da = dq + (x * 2 * kAtomStep + off), db = dk + ((u >> 1 & 1) * 2 * kAtomStep + (u & 1) * kHalfStep + off);
+                        if (ks == 0) umma_bf16_ss<false>(128 * x + 64 * (u & 1), da, db, idesc_s);
+                        else umma_bf16_ss<true>(128 * x + 64 * (u & 1), da, db, idesc_s);
+                    }
+                    umma_commit(&s_full[2 * x + (u & 1)]);
+                    if (last) umma_commit(&k_free[u >> 1 & 1]);
+                }
+                __syncwarp();
+            };
+            auto values = [&](int x, int u, bool first, bool last) {
+                if (elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {   // 16 keys: 8 columns of weights, 2048 bytes of V
+                        const uint64_t db = dv + ((u >> 1 & 1) * 2 * kAtomStep + (u & 1) * kHalfStep + ks * (2048 >> 4));
+                        if (ks == 0 && first) umma_bf16_ts<false>(kColO + 128 * x, 128 * x + 64 * (u & 1) + 8 * ks, db, idesc_o);
+                        else umma_bf16_ts<true>(kColO + 128 * x, 128 * x + 64 * (u & 1) + 8 * ks, db, idesc_o);
+                    }
+                    umma_commit(&pv_done[x]);
+                    if (last) umma_commit(&v_free[u >> 1 & 1]);
+                }
+                __syncwarp();
+            };
+            bool ok = wait(q_full, 0u, 83) && wait(&k_full[0], 0u, 83);
+            if (ok) {
+                tc_fence_after_sync();
+                scores(0, 0, !both && n == 1);
+                if (both) scores(1, 0, n == 1);
+                if (n > 1) {
+                    scores(0, 1, !both);
+                    if (both) scores(1, 1, true);
+                }
+            }
+            // A wait costs some 150 cycles even when it is over: each stands right behind products that were just issued.
+            for (uint32_t h0 = 0; ok && h0 < n; h0 += 4) {
+                const uint32_t phase = h0 >> 2 & 1;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t h = h0 + u;
+                    if (!ok || h >= n) break;
+                    if (!(ok = wait(&p_full[u & 1], u >> 1, 84))) break;
+                    if (!(u & 1) && !(ok = wait(&v_full[u >> 1], phase, 85))) break;
+                    tc_fence_after_sync();
+                    const bool more = h + 2 < n, ends = (u & 1) || h + 1 == n, next_ends = (u & 1) || h + 3 == n;
+                    values(0, u, u == 0 && h0 == 0, !both && ends);
+                    if (both && !(ok = wait(&p_full[2 + (u & 1)], u >> 1, 84))) break;
+                    if (more && !(u & 1) && !(ok = wait(&k_full[u >> 1 ^ 1], u ? phase ^ 1u : phase, 86))) break;
+                    tc_fence_after_sync();
+                    if (more) scores(0, u + 2, !both && next_ends);
+                    if (both) {
+                        values(1, u, u == 0 && h0 == 0, ends);
+                        if (more) scores(1, u + 2, next_ends);
+                    }
+                }
+            }
+            if (*abort_flag) {   // no product may still be writing tensor memory when it is freed
+                if (elect_one()) umma_commit(drain_bar);
+                __syncwarp();
+                mbar_wait(drain_bar, 0u, never_flag, a.status, 87);
+            }
+        }
+    } else {
+        // -------------------------------------------------------------------------------- softmax: one thread per pair
+        const uint32_t x = warp >> 2, p = tid;       // tile; pair of the CTA
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16), col_o = lanes + kColO + 128 * x;
+        bool ok = x == 0 || two;
+        if (ok && halves) {
+            // q of the warp's 32 pairs: 8 bytes a lane and row, 16 rows on their way together; bf16 rows are brought into fp16's range as in kv8_attn.cu
+#pragma unroll 1
+            for (uint32_t p0 = 32 * warp; p0 < 32 * warp + 32; p0 += 16) {
+                uint2 v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t pair = pair0 + p0 + i, of = kv8_row_of(a, pair), row = r.start + of, h = kvh * a.group + pair - of * a.group;
+                    v[i] = p0 + i < here ? *reinterpret_cast<const uint2*>(a.q + static_cast<size_t>(row) * a.ldq + static_cast<size_t>(h) * HD + 4 * lane) : make_uint2(0, 0);
+                }
+                uint32_t top[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top[i] = kv8_query_top<1>(&v[i]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t row = (p0 + i) & 127;
+                    const float up = kv8_query_row<Act, 1>(&v[i], top[i]);
+                    if (lane == 0) rank[p0 + i] = up;
+                    // columns 4 lane ..: half lane / 16, 16-byte piece (lane / 2) % 8, swizzled by the row
+                    *reinterpret_cast<uint2*>(smem + Smem::kQ + (x * 2 + (lane >> 4)) * Smem::kAtom + row * 128 + ((((lane >> 1) & 7) ^ (row & 7)) << 4) + (lane & 1) * 8) = v[i];
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const bool on = p < here, runs = ok;
+        const float mul = ok && halves ? a.scale * rank[p] : 0.f;
+        const uint32_t see = on ? seen[p] : most;    // pairs past the last are computed (their q is zero) and not stored
+        float m = kKv8None, l = 0.f;
+        for (uint32_t h = 0; ok && h < halves; ++h) {
+            if (!(ok = mbar_wait(&scale_full[(h >> 1) % kScaleSlots], (h >> 1) / kScaleSlots & 1u, abort_flag, a.status, 88))) break;
+            if (!(ok = mbar_wait(&s_full[2 * x + (h & 1)], h >> 1 & 1, abort_flag, a.status, 89))) break;
+            __syncwarp();
+            tc_fence_after_sync();
+            const float4* sc = scales + (h >> 1) % kScaleSlots * 8 + 4 * (h & 1);
+            const uint32_t key = key0 + h * kHalf, col_s = lanes + 128 * x + 64 * (h & 1);
+            const int vis = static_cast<int>(min(see, key + kHalf)) - static_cast<int>(min(see, key));   // of the 64 keys
+            auto settled = [&] {   // the V product of the last 64 keys (the one before it came before these scores)
+                const bool done = mbar_wait(&pv_done[x], (h - 1) & 1u, abort_flag, a.status, 91);
+                __syncwarp();
+                tc_fence_after_sync();
+                return done;
+            };
+            if (__any_sync(0xffffffffu, vis < static_cast<int>(kHalf))) ok = softmax_half<true>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
+            else ok = softmax_half<false>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
+            if (!ok) break;
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * x + (h & 1)]);
+        }
+        if (ok && runs && !idle) {
+            // A tile's q is free once its last product is done (its scores came before it): a warp's 32 rows go through 8 KB of it, 64 columns
+            // at a time, so that rows leave in whole pieces. Row r keeps its 16-byte pieces at piece ^ (r % 16).
+            // The last two V products, one after the other: the one before them is done (the last scores came after it), and a wait may
+            // not look further ahead than one phase.
+            bool there = halves < 2 || mbar_wait(&pv_done[x], (halves - 2) & 1u, abort_flag, a.status, 90);
+            if (there && halves) there = mbar_wait(&pv_done[x], (halves - 1) & 1u, abort_flag, a.status, 90);
+            if (there) {
+                __syncwarp();
+                tc_fence_after_sync();
+                uint8_t* stage = smem + Smem::kQ + warp * 8192;
+                const float by = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+                const uint32_t first = 32 * warp, col8 = lane & 7;           // pair of the CTA that lane 0 holds; eight lanes a row
+                float* parts = a.part + (static_cast<size_t>(tile_id) * a.chunks + z) * kPairs * kLd;
+                if (!whole && on) *reinterpret_cast<float2*>(parts + p * kLd + HD) = make_float2(m, l);
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    __syncwarp();
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        uint32_t v[16];
+                        if (halves) {
+                            tmem_ld_32x32_x16(col_o + 64 * c + 16 * q4, v);
+                            tmem_ld_wait();
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            uint4 o = make_uint4(0, 0, 0, 0);
+                            if (halves) o = make_uint4(__float_as_uint(__uint_as_float(v[e]) * by), __float_as_uint(__uint_as_float(v[e + 1]) * by),
+                                                       __float_as_uint(__uint_as_float(v[e + 2]) * by), __float_as_uint(__uint_as_float(v[e + 3]) * by));
+                            *reinterpret_cast<uint4*>(stage + lane * 256 + (((4 * q4 + e / 4) ^ (lane & 15)) << 4)) = o;
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {                       // four rows at a time
+                        const uint32_t rr = 4 * i + (lane >> 3), pr = first + rr, d = 64 * c + 8 * col8;
+                        const float4 o0 = *reinterpret_cast<const float4*>(stage + rr * 256 + (((2 * col8) ^ (rr & 15)) << 4));
+                        const float4 o1 = *reinterpret_cast<const float4*>(stage + rr * 256 + (((2 * col8 + 1) ^ (rr & 15)) << 4));
+                        if (pr >= here) continue;
+                        if (whole) {
+                            kv8_store8<Act>(a, r, pair0 + pr, kvh, d, HD, o0, o1);
+                        } else {
+                            *reinterpret_cast<float4*>(parts + pr * kLd + d) = o0;
+                            *reinterpret_cast<float4*>(parts + pr * kLd + d + 4) = o1;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // ------------------------------------------------------------------------------------ teardown
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after_sync();
+        __syncwarp();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// Joins the chunks of 16 pairs of a tile, in chunk order; a thread takes 8 columns of a pair. Tiles that one chunk held are done already.
+template <typename Act>
+__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Args a) {
+    const uint32_t tile_id = blockIdx.x / (kPairs / 16), p = blockIdx.x % (kPairs / 16) * 16 + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+    const uint32_t kvh = tile_id % a.c.nkv, mt = a.tiles - 1 - tile_id / a.c.nkv % a.tiles, j = tile_id / a.c.nkv / a.tiles;
+    const Kv8Rows r = kv8_rows(a.c, a.q_start, j, a.rows, a.max_q);
+    if (!r.ok || r.len > a.max_len) return;
+    const uint32_t pair0 = mt * kPairs, pairs = r.count * a.group;
+    if (pair0 >= pairs) return;
+    const uint32_t here = min(static_cast<uint32_t>(kPairs), pairs - pair0);
+    __shared__ uint32_t most_at;
+    if (threadIdx.x == 0) most_at = 0;
+    __syncthreads();
+    bool past = false;
+    uint32_t n = threadIdx.x < here ? kv8_visible(r, a.qpos, kv8_row_of(a, pair0 + threadIdx.x), &past) : 0u;
+    n = __reduce_max_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) atomicMax(&most_at, n);
+    __syncthreads();
+    const uint32_t most = most_at;
+    if (most <= a.chunk || p >= here) return;
+    const uint32_t chunks = (most + a.chunk - 1) / a.chunk;
+    const float* from = a.part + (static_cast<size_t>(tile_id) * a.chunks * kPairs + p) * kLd;
+    constexpr size_t kStepFloats = static_cast<size_t>(kPairs) * kLd;
+    float top = kKv8None, total = 0.f, x[8] = {};
+    for (uint32_t k = 0; k < chunks; ++k) top = fmaxf(top, from[k * kStepFloats + HD]);
+#pragma unroll 4
+    for (uint32_t k = 0; k < chunks; ++k) {
+        const float* at = from + k * kStepFloats;
+        const float2 ml = *reinterpret_cast<const float2*>(at + HD);
+        const float4 u = *reinterpret_cast<const float4*>(at + d), w = *reinterpret_cast<const float4*>(at + d + 4);
+        const float by = ex2(ml.x - top), v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+        total = fmaf(ml.y, by, total);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(v[i], by, x[i]);
+    }
+    kv8_finish<Act>(a, r, pair0 + p, kvh, d, HD, total, x);
+}
+
+}  // namespace
+
+int dc_kv8_attention_tc_warm(dc_ctx* ctx) {
+    static bool set[16] = {};
+    if (set[ctx->device & 15]) return DC_OK;
+    cudaError_t e = cudaFuncSetAttribute(kv8_attn_tc_kernel<ActF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Smem::kBytes));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv8_attn_tc_kernel<ActBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Smem::kBytes));
+    if (e != cudaSuccess) return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention: cannot opt in to %u bytes of shared memory: %s", Smem::kBytes, cudaGetErrorString(e));
+    set[ctx->device & 15] = true;
+    return DC_OK;
+}
+
+// How a call is cut: tiles of 256 pairs; where there are fewer of them than SMs, the keys in chunks of at least two steps.
+Kv8Cut dc_kv8_attention_tc_cut(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
+    Kv8Cut t;
+    const uint64_t pairs = static_cast<uint64_t>(max_q) * (nq / c->nkv);
+    t.tiles = static_cast<uint32_t>((pairs + kPairs - 1) / kPairs);
+    const uint64_t whole = static_cast<uint64_t>(c->n_seqs) * c->nkv * t.tiles;
+    uint64_t parts = static_cast<uint64_t>(ctx->sm_count) / whole;
+    const uint64_t most = (max_len + 2 * kKeys - 1) / (2 * kKeys);
+    parts = parts < 1 ? 1 : parts > most ? most : parts;
+    t.chunk = static_cast<uint32_t>(((max_len + parts - 1) / parts + kKeys - 1) / kKeys * kKeys);
+    t.chunks = (max_len + t.chunk - 1) / t.chunk;
+    t.ctas = whole * t.chunks;
+    t.part_bytes = t.chunks > 1 ? t.ctas * kPairs * kLd * sizeof(float) : 0;
+    return t;
+}
+
+int dc_kv8_attention_tc(dc_ctx* ctx, cudaStream_t s, const dc::Kv8Args& a, uint64_t ctas) {
+    const int rc = dc_kv8_attention_tc_warm(ctx);
+    if (rc != DC_OK) return rc;
+    const bool f16 = ctx->act_dtype == DC_ACT_F16;
+    auto kern = f16 ? kv8_attn_tc_kernel<ActF16> : kv8_attn_tc_kernel<ActBF16>;
+    kern<<<static_cast<uint32_t>(ctas), kThreads, Smem::kBytes, s>>>(a);
+    const int launched = dc_check_launch(ctx, "kv8_attention (tcgen05)");
+    if (launched != DC_OK || a.chunks == 1) return launched;
+    auto join = f16 ? kv8_join_kernel<ActF16> : kv8_join_kernel<ActBF16>;
+    join<<<static_cast<uint32_t>(ctas / a.chunks * (kPairs / 16)), 256, 0, s>>>(a);
+    return dc_check_launch(ctx, "kv8_attention (join)");
+}
