@@ -420,7 +420,8 @@ class Kv8(_Family):
     `stream` None is the current stream of the context's device."""
 
     def _stream(self, stream) -> int:
-        return torch.cuda.current_stream(self.dev.device).cuda_stream if stream is None else _stream(stream)
+        # the handle of torch's current stream without a Stream object around it: 0.1 us instead of 1.3, a fifth of a short call
+        return torch._C._cuda_getCurrentRawStream(self.dev.device) if stream is None else _stream(stream)
 
     def extend(self, stream, cache: Kv8Cache, add):
         """Lengthens sequence j by add[j] tokens: gives it the pages it lacks."""
