@@ -32,8 +32,9 @@ __host__ __device__ inline Plan plan_at(void* ws, uint32_t n_pages) {
     return p;
 }
 
-// Exclusive prefix sum over the block's threads; *total gets the sum of all. `sums`: 33 words of shared memory.
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums, uint32_t* total) {
+// Exclusive prefix sum over the block's threads; *total gets the sum of all. One barrier: every warp adds up the warps' sums for itself.
+// `sums`: 2 x 32 words of shared memory, used in turn (`turn` counts the calls), so that a call does not wait for the last one's readers.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums, uint32_t& turn, uint32_t* total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t s = x;
 #pragma unroll
@@ -41,27 +42,23 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums, uint3
         const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += y;
     }
-    if (lane == 31) sums[warp] = s;
+    uint32_t* mine = sums + 32 * (turn++ & 1u);
+    if (lane == 31) mine[warp] = s;
     __syncthreads();
-    if (warp == 0) {
-        uint32_t t = sums[lane];
+    uint32_t t = mine[lane];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, t, o);
-            if (lane >= o) t += y;
-        }
-        sums[lane] = t;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += y;
     }
-    __syncthreads();
-    const uint32_t before = warp ? sums[warp - 1] : 0u;
-    *total = sums[31];
-    __syncthreads();
-    return before + s - x;
+    *total = __shfl_sync(0xffffffffu, t, 31);
+    const uint32_t before = __shfl_sync(0xffffffffu, t, max(warp - 1, 0));
+    return (warp ? before : 0u) + s - x;
 }
 
 // The first `need` pages with refs 0, ascending, into slots; returns how many there are, at most `need`. The caller's writes to refs
 // are behind a barrier.
-__device__ uint32_t find_free(const uint32_t* refs, uint32_t n_pages, uint32_t need, uint32_t* slots, uint32_t* sums) {
+__device__ uint32_t find_free(const uint32_t* refs, uint32_t n_pages, uint32_t need, uint32_t* slots, uint32_t* sums, uint32_t& turn) {
     uint32_t found = 0;
     for (uint32_t base = 0; base < n_pages && found < need; base += 4 * kPlanThreads) {
         const uint32_t at = base + 4 * threadIdx.x;
@@ -70,7 +67,7 @@ __device__ uint32_t find_free(const uint32_t* refs, uint32_t n_pages, uint32_t n
         for (int i = 0; i < 4; ++i)
             if (at + i < n_pages && __ldcg(refs + at + i) == 0u) mask |= 1u << i;
         uint32_t total;
-        uint32_t place = found + block_scan(__popc(mask), sums, &total);
+        uint32_t place = found + block_scan(__popc(mask), sums, turn, &total);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (mask >> i & 1u) {
@@ -85,72 +82,75 @@ __device__ uint32_t find_free(const uint32_t* refs, uint32_t n_pages, uint32_t n
 // A sequence's pages, from its length as it is now; flags a length that its row of the table cannot hold.
 __device__ __forceinline__ bool length_fits(const dc_kv8_cache& c, uint32_t len) { return len <= c.max_pages * c.page_size; }
 
-// The pages of sequences ids[0 .. n): refs - 1 (give_back: + 1 again). Warps take the sequences in turn. Returns nothing; *bad is set
-// when a page that nobody held is given up (it stays at 0).
-__device__ void release(const dc_kv8_cache& c, const uint32_t* ids, uint32_t n, bool give_back, int* bad) {
+// The copying kernel is launched while the deciding one runs (programmatic dependent launch) and waits for it here.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_launcher() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// refs of the pages of sequences ids[0 .. n): `by` = -1 gives them up, + 1 takes them back. Warps take the sequences in turn. *bad is set
+// where a page id is outside the pool (it is passed over) or a page that nobody held is given up.
+__device__ __forceinline__ void release(const dc_kv8_cache& c, const uint32_t* ids, uint32_t n, int by, int* bad) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (uint32_t i = warp; i < n; i += kPlanThreads / 32) {
         const uint32_t j = ids[i], pages = kv8_pages(c.lens[j], c.page_size);
         for (uint32_t col = lane; col < pages; col += 32) {
             const uint32_t page = c.table[static_cast<size_t>(j) * c.max_pages + col];
-            if (give_back) atomicAdd(&c.refs[page], 1u);
-            else if (atomicSub(&c.refs[page], 1u) == 0u) *bad = DC_STATUS_KV8_REFS;
+            if (page >= c.n_pages) *bad = DC_STATUS_KV8_PAGE;
+            else if (atomicAdd(&c.refs[page], static_cast<uint32_t>(by)) == 0u && by < 0) *bad = DC_STATUS_KV8_REFS;
         }
     }
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
 extend_kernel(dc_kv8_cache c, const uint32_t* __restrict__ add, Plan plan, int* __restrict__ status) {
-    __shared__ uint32_t sums[33];
+    __shared__ uint32_t sums[64];
     __shared__ int bad;
+    uint32_t turn = 0;
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
-    // what each sequence lacks; `slots` first receives the free pages, so the needs are scanned twice rather than kept
-    uint32_t need = 0;
-    for (uint32_t base = 0; base < c.n_seqs; base += kPlanThreads) {
+    // what each sequence lacks, and how many pages the ones before it in the round lack
+    uint32_t need = 0, held = 0, mine = 0, len = 0, more = 0, place = 0;
+    auto look = [&](uint32_t base, uint32_t* total) {
         const uint32_t j = base + threadIdx.x;
-        uint32_t mine = 0;
+        held = mine = len = more = 0;
         if (j < c.n_seqs) {
-            const uint64_t len = c.lens[j], after = len + add[j];
-            if (after > static_cast<uint64_t>(c.max_pages) * c.page_size) bad = DC_STATUS_KV8_LENGTH;
-            else mine = kv8_pages(static_cast<uint32_t>(after), c.page_size) - kv8_pages(static_cast<uint32_t>(len), c.page_size);
+            len = c.lens[j];
+            more = add[j];
+            const uint64_t after = static_cast<uint64_t>(len) + more;
+            if (after > static_cast<uint64_t>(c.max_pages) * c.page_size) {
+                bad = DC_STATUS_KV8_LENGTH;
+            } else {
+                held = kv8_pages(len, c.page_size);
+                mine = kv8_pages(static_cast<uint32_t>(after), c.page_size) - held;
+            }
         }
+        // 1024 of at most 2^21 + 1 each: fits 32 bits
+        return block_scan(min(mine, c.n_pages + 1), sums, turn, total);
+    };
+    for (uint32_t base = 0; base < c.n_seqs; base += kPlanThreads) {
         uint32_t total;
-        block_scan(min(mine, c.n_pages + 1), sums, &total);   // 1024 of at most 2^21 + 1 each: fits 32 bits
-        need = min(need + total, c.n_pages + 1);              // more than the pool is too many, however many
-    }
-    if (!bad && need > c.n_pages) {
-        __syncthreads();
-        if (threadIdx.x == 0) bad = DC_STATUS_KV8_POOL;
+        place = look(base, &total);
+        need = min(need + total, c.n_pages + 1);   // more than the pool is too many, however many
     }
     __syncthreads();
-    if (bad) {
-        if (threadIdx.x == 0) kv8_flag(status, bad);
-        return;
-    }
-    if (find_free(c.refs, c.n_pages, need, plan.slots, sums) < need) {
-        if (threadIdx.x == 0) kv8_flag(status, DC_STATUS_KV8_POOL);
+    if (bad || need > c.n_pages || find_free(c.refs, c.n_pages, need, plan.slots, sums, turn) < need) {
+        if (threadIdx.x == 0) kv8_flag(status, bad ? bad : DC_STATUS_KV8_POOL);
         return;
     }
     __syncthreads();
     uint32_t given = 0;
     for (uint32_t base = 0; base < c.n_seqs; base += kPlanThreads) {
-        const uint32_t j = base + threadIdx.x;
-        uint32_t held = 0, mine = 0, len = 0;
-        if (j < c.n_seqs) {
-            len = c.lens[j];
-            held = kv8_pages(len, c.page_size);
-            mine = kv8_pages(len + add[j], c.page_size) - held;
+        if (c.n_seqs > kPlanThreads) {   // otherwise the one round above still stands
+            uint32_t total;
+            place = given + look(base, &total);
+            given += total;
         }
-        uint32_t total;
-        const uint32_t place = given + block_scan(mine, sums, &total);
+        const uint32_t j = base + threadIdx.x;
         for (uint32_t i = 0; i < mine; ++i) {
             const uint32_t page = plan.slots[place + i];
             c.table[static_cast<size_t>(j) * c.max_pages + held + i] = page;
             c.refs[page] = 1u;
         }
-        if (j < c.n_seqs) c.lens[j] = len + add[j];
-        given += total;
+        if (j < c.n_seqs) c.lens[j] = len + more;
     }
 }
 
@@ -162,65 +162,78 @@ __device__ __forceinline__ uint32_t copied_pages(const dc_kv8_cache& c, uint32_t
 __global__ void __launch_bounds__(kPlanThreads)
 fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __restrict__ dst, uint32_t n, bool deep, Plan plan, int* __restrict__ status) {
     extern __shared__ uint32_t taken[];   // one bit a sequence: it is a destination
-    __shared__ uint32_t sums[33];
+    __shared__ uint32_t sums[64];
     __shared__ int bad;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t turn = 0;
+    launch_dependents();
     for (uint32_t i = threadIdx.x; i < (c.n_seqs + 31) / 32; i += kPlanThreads) taken[i] = 0u;
     if (threadIdx.x == 0) {
         bad = 0;
         plan.head[0] = 0u;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
-        const uint32_t d = dst[i];
-        if (d >= c.n_seqs || (atomicOr(&taken[d >> 5], 1u << (d & 31)) >> (d & 31) & 1u)) bad = DC_STATUS_KV8_SEQUENCE;
-        else if (!length_fits(c, c.lens[d])) bad = DC_STATUS_KV8_LENGTH;
-    }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
-        const uint32_t s = src[i];
-        if (s >= c.n_seqs || (taken[s >> 5] >> (s & 31) & 1u)) bad = DC_STATUS_KV8_SEQUENCE;
-        else if (!length_fits(c, c.lens[s])) bad = DC_STATUS_KV8_LENGTH;
-    }
-    __syncthreads();
-    if (!bad)   // every page id that will be read below names a page
-        for (uint32_t i = warp; i < 2 * n; i += kPlanThreads / 32) {
-            const uint32_t j = i < n ? src[i] : dst[i - n], pages = kv8_pages(c.lens[j], c.page_size);
-            for (uint32_t col = lane; col < pages; col += 32)
-                if (c.table[static_cast<size_t>(j) * c.max_pages + col] >= c.n_pages) bad = DC_STATUS_KV8_PAGE;
+    // what the forks name, and how many pages they copy: `place` of them before this thread's in the round
+    uint32_t need = 0, place = 0;
+    for (uint32_t base = 0; base < n; base += kPlanThreads) {
+        const uint32_t i = base + threadIdx.x;
+        uint32_t copied = 0, total;
+        if (i < n) {
+            const uint32_t d = dst[i], s = src[i];
+            if (d >= c.n_seqs || s >= c.n_seqs) {
+                bad = DC_STATUS_KV8_SEQUENCE;
+            } else {
+                const uint32_t d_len = c.lens[d], s_len = c.lens[s];
+                if (atomicOr(&taken[d >> 5], 1u << (d & 31)) >> (d & 31) & 1u) bad = DC_STATUS_KV8_SEQUENCE;
+                if (!length_fits(c, d_len) || !length_fits(c, s_len)) bad = DC_STATUS_KV8_LENGTH;
+                else copied = min(copied_pages(c, s_len, deep), c.n_pages + 1);
+            }
         }
+        place = block_scan(copied, sums, turn, &total);
+        need = min(need + total, c.n_pages + 1);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n && !bad; i += kPlanThreads) {
+        const uint32_t s = src[i];
+        if (taken[s >> 5] >> (s & 31) & 1u) bad = DC_STATUS_KV8_SEQUENCE;
+    }
     __syncthreads();
     if (bad) {
         if (threadIdx.x == 0) kv8_flag(status, bad);
         return;
     }
-    uint32_t need = 0;
-    for (uint32_t base = 0; base < n; base += kPlanThreads) {
-        const uint32_t i = base + threadIdx.x;
-        uint32_t total;
-        block_scan(i < n ? min(copied_pages(c, c.lens[src[i]], deep), c.n_pages + 1) : 0u, sums, &total);
-        need = min(need + total, c.n_pages + 1);
+    // the destinations give up what they hold; what the sources hold has to name pages
+    release(c, dst, n, -1, &bad);
+    for (uint32_t i = warp; i < n; i += kPlanThreads / 32) {
+        const uint32_t j = src[i], pages = kv8_pages(c.lens[j], c.page_size);
+        for (uint32_t col = lane; col < pages; col += 32)
+            if (c.table[static_cast<size_t>(j) * c.max_pages + col] >= c.n_pages) bad = DC_STATUS_KV8_PAGE;
     }
-    release(c, dst, n, false, &bad);
     __syncthreads();
-    const bool enough = need <= c.n_pages && !bad && find_free(c.refs, c.n_pages, need, plan.slots, sums) == need;
+    const bool enough = !bad && need <= c.n_pages && find_free(c.refs, c.n_pages, need, plan.slots, sums, turn) == need;
     __syncthreads();
     if (!enough) {   // as it was
-        release(c, dst, n, true, &bad);
-        if (threadIdx.x == 0) kv8_flag(status, bad ? bad : DC_STATUS_KV8_POOL);
+        const int what = bad ? bad : DC_STATUS_KV8_POOL;
+        __syncthreads();
+        release(c, dst, n, 1, &bad);
+        if (threadIdx.x == 0) kv8_flag(status, what);
         return;
     }
     uint32_t given = 0;
     for (uint32_t base = 0; base < n; base += kPlanThreads) {
-        const uint32_t i = base + threadIdx.x;
-        uint32_t total;
-        const uint32_t place = given + block_scan(i < n ? copied_pages(c, c.lens[src[i]], deep) : 0u, sums, &total);
-        // warp by warp: the 32 forks of this warp in turn, lanes over the pages
-        for (int k = 0; k < 32; ++k) {
-            const uint32_t at = base + 32 * warp + k;
-            if (at >= n) break;
-            const uint32_t s = src[at], len = c.lens[s], pages = kv8_pages(len, c.page_size), copied = copied_pages(c, len, deep), shared = pages - copied;
-            const uint32_t first = __shfl_sync(0xffffffffu, place, k);
+        if (n > kPlanThreads) {   // otherwise the one round above still stands
+            const uint32_t i = base + threadIdx.x;
+            uint32_t total;
+            place = given + block_scan(i < n ? copied_pages(c, c.lens[src[i]], deep) : 0u, sums, turn, &total);
+            given += total;
+        }
+        // warps over the round's forks, lanes over the pages; a fork's place comes from the warp that scanned it
+        __shared__ uint32_t places[kPlanThreads];
+        __syncthreads();
+        places[threadIdx.x] = place;
+        __syncthreads();
+        for (uint32_t k = warp; k < kPlanThreads && base + k < n; k += kPlanThreads / 32) {
+            const uint32_t at = base + k, s = src[at], len = c.lens[s], pages = kv8_pages(len, c.page_size), copied = copied_pages(c, len, deep), shared = pages - copied;
             const uint32_t* from = c.table + static_cast<size_t>(s) * c.max_pages;
             uint32_t* to = c.table + static_cast<size_t>(dst[at]) * c.max_pages;
             for (uint32_t col = lane; col < pages; col += 32) {
@@ -228,7 +241,7 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
                 if (col < shared) {
                     atomicAdd(&c.refs[page], 1u);
                 } else {
-                    const uint32_t slot = first + col - shared, fresh = plan.slots[slot];
+                    const uint32_t slot = places[k] + col - shared, fresh = plan.slots[slot];
                     plan.moves[slot] = make_uint2(page, fresh);
                     c.refs[fresh] = 1u;
                     page = fresh;
@@ -236,7 +249,6 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
                 to[col] = page;
             }
         }
-        given += total;
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) c.lens[dst[i]] = c.lens[src[i]];
@@ -266,31 +278,44 @@ __global__ void __launch_bounds__(128) free_kernel(dc_kv8_cache c, const uint32_
 }
 
 __global__ void __launch_bounds__(kPlanThreads) compact_kernel(dc_kv8_cache c, Plan plan, uint32_t* __restrict__ live_out) {
-    __shared__ uint32_t sums[33];
-    uint32_t live = 0;
-    for (uint32_t base = 0; base < c.n_pages; base += 4 * kPlanThreads) {
-        uint32_t mine = 0, total;
+    __shared__ uint32_t sums[64];
+    uint32_t turn = 0, live = 0, mask = 0;   // of four pages, those in use
+    launch_dependents();
+    auto look = [&](uint32_t at) {
+        mask = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t p = base + 4 * threadIdx.x + i;
-            if (p < c.n_pages && c.refs[p] != 0u) ++mine;
-        }
-        block_scan(mine, sums, &total);
+        for (int i = 0; i < 4; ++i)
+            if (at + i < c.n_pages && c.refs[at + i] != 0u) mask |= 1u << i;
+    };
+    for (uint32_t base = 0; base < c.n_pages; base += 4 * kPlanThreads) {
+        uint32_t total;
+        look(base + 4 * threadIdx.x);
+        block_scan(__popc(mask), sums, turn, &total);
         live += total;
     }
-    // as many pages in use at or past `live` as free ones below it: the i-th goes to the i-th
+    // as many pages in use at or past `live` as free ones below it: the i-th goes to the i-th. A round has at most 4096 of either: one
+    // scan adds up both, 16 bits each
     uint32_t holes = 0, movers = 0;
-    for (uint32_t base = 0; base < c.n_pages; base += kPlanThreads) {
-        const uint32_t p = base + threadIdx.x;
-        const bool held = p < c.n_pages && c.refs[p] != 0u;
-        const bool hole = p < live && !held, mover = p >= live && held;
-        uint32_t holes_here, movers_here;
-        const uint32_t h = holes + block_scan(hole, sums, &holes_here), m = movers + block_scan(mover, sums, &movers_here);
-        if (hole) plan.moves[h].y = p;
-        if (mover) plan.moves[m].x = p;
-        if (p < c.n_pages) plan.slots[p] = p;
-        holes += holes_here;
-        movers += movers_here;
+    for (uint32_t base = 0; base < c.n_pages; base += 4 * kPlanThreads) {
+        const uint32_t at = base + 4 * threadIdx.x;
+        if (c.n_pages > 4 * kPlanThreads) look(at);   // otherwise the one round above still stands
+        uint32_t hole = 0, mover = 0, total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (at + i < c.n_pages) {
+                if (at + i < live && !(mask >> i & 1u)) hole |= 1u << i;
+                if (at + i >= live && (mask >> i & 1u)) mover |= 1u << i;
+                plan.slots[at + i] = at + i;
+            }
+        const uint32_t both = block_scan(__popc(hole) | __popc(mover) << 16, sums, turn, &total);
+        uint32_t h = holes + (both & 0xffffu), m = movers + (both >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (hole >> i & 1u) plan.moves[h++].y = at + i;
+            if (mover >> i & 1u) plan.moves[m++].x = at + i;
+        }
+        holes += total & 0xffffu;
+        movers += total >> 16;
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < movers; i += kPlanThreads) {
@@ -309,6 +334,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(dc_kv8_cache c, P
 // page_size * hd codes and a scale. No page is both read and written (the lists are made so).
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(dc_kv8_cache c, Plan plan, bool rename, int* __restrict__ status) {
     const uint32_t lane = threadIdx.x & 31;
+    wait_for_launcher();
     const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kCopyThreads / 32);
     const uint64_t units = static_cast<uint64_t>(plan.head[0]) * c.layers * 2 * c.nkv;
     const uint32_t per_row = c.hd / 16, vectors = c.page_size * per_row;
@@ -361,6 +387,25 @@ uint32_t copy_grid(const dc_ctx* ctx, const dc_kv8_cache* c, uint64_t moves) {
     const uint64_t units = moves * c->layers * 2 * c->nkv, ctas = (units + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
     const uint64_t most = static_cast<uint64_t>(ctx->sm_count) * 8;
     return static_cast<uint32_t>(ctas < 1 ? 1 : ctas < most ? ctas : most);
+}
+
+// Launches the copying kernel so that it may start while the deciding one, enqueued just before, still runs.
+int launch_copies(dc_ctx* ctx, cudaStream_t s, const char* what, uint32_t grid, const dc_kv8_cache& c, Plan plan, bool rename) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kCopyThreads);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, copy_kernel, c, plan, rename, ctx->status_dev);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return dc_fail(ctx, DC_CUDA_ERROR, "%s: launch failed: %s", what, cudaGetErrorString(e));
+    }
+    return dc_check_launch(ctx, what);
 }
 
 int pages_begin(dc_ctx* ctx, const char* who, const dc_kv8_cache* cache, Plan* plan) {
@@ -448,8 +493,7 @@ extern "C" int dc_kv8_fork(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache,
     fork_kernel<<<1, kPlanThreads, (cache->n_seqs + 31) / 32 * 4, s>>>(*cache, src, dst, n, deep != 0, plan, ctx->status_dev);
     if ((rc = dc_check_launch(ctx, "kv8_fork")) != DC_OK) return rc;
     const uint64_t most = deep ? static_cast<uint64_t>(n) * cache->max_pages : n;
-    copy_kernel<<<copy_grid(ctx, cache, most < cache->n_pages ? most : cache->n_pages), kCopyThreads, 0, s>>>(*cache, plan, false, ctx->status_dev);
-    return dc_check_launch(ctx, "kv8_fork (copies)");
+    return launch_copies(ctx, s, "kv8_fork (copies)", copy_grid(ctx, cache, most < cache->n_pages ? most : cache->n_pages), *cache, plan, false);
 }
 
 extern "C" int dc_kv8_free(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, const uint32_t* seqs, uint32_t n) {
@@ -474,6 +518,5 @@ extern "C" int dc_kv8_compact(dc_ctx* ctx, void* stream, const dc_kv8_cache* cac
     compact_kernel<<<1, kPlanThreads, 0, s>>>(*cache, plan, live);
     if ((rc = dc_check_launch(ctx, "kv8_compact")) != DC_OK) return rc;
     // at most half of the pages move
-    copy_kernel<<<copy_grid(ctx, cache, cache->n_pages / 2 + 1), kCopyThreads, 0, s>>>(*cache, plan, true, ctx->status_dev);
-    return dc_check_launch(ctx, "kv8_compact (copies)");
+    return launch_copies(ctx, s, "kv8_compact (copies)", copy_grid(ctx, cache, cache->n_pages / 2 + 1), *cache, plan, true);
 }
