@@ -501,7 +501,7 @@ uint32_t longest(const dc_kv8_cache* c, uint32_t max_len) {
 // tcgen05 and here: 64 pairs over 2,307 keys 18 and 13, over 16,000 keys 32 and 46; 64 sequences of 64 pairs over 1,200 keys 171
 // and 132; 256 pairs over 2,307 keys 24 and 24, over 16,000 keys 42 and 124; 16 sequences of 256 pairs over 1,500 keys 64 and 150.
 bool on_tcgen05(const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
-    return c->hd == 128 && static_cast<uint64_t>(max_q) * (nq / c->nkv) >= (max_len < 8192 ? 128 : 64);
+    return static_cast<uint64_t>(max_q) * (nq / c->nkv) >= (max_len < 8192 ? 128 : 64);
 }
 
 }  // namespace

@@ -77,13 +77,17 @@ __device__ __forceinline__ uint32_t kv8_row_of(const Kv8Args& a, uint32_t pair) 
 // much in the total and little in the product.
 __device__ __forceinline__ float kv8_total(float exact, float rounded) { return exact >= 6.103515625e-05f ? rounded : exact; }
 
-// The largest magnitude of a query row, as 16 bits; WORDS 8-byte pieces a lane holds of it.
+// The largest magnitude of a query row, as 16 bits; WORDS 8-byte pieces a lane holds of it, `lanes` (16 or 32) lanes hold the row.
 template <int WORDS>
-__device__ __forceinline__ uint32_t kv8_query_top(const uint2* x) {
+__device__ __forceinline__ uint32_t kv8_query_top(const uint2* x, int lanes = 32) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) top = __vmaxu2(top, __vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu));
-    return __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    top = max(top & 0xffffu, top >> 16);
+    if (lanes == 32) return __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
 }
 // A bf16 row is divided by a power of two that brings its largest magnitude to [2^14, 2^15): then its 8 bits fit fp16 but for elements
 // 2^-28 below it. fp16 rows stay as they are. Returns the divisor; NaN for a row that is not finite.
@@ -106,24 +110,32 @@ __device__ __forceinline__ float kv8_query_row(uint2* x, uint32_t top) {
     return Act::one(static_cast<uint16_t>(top)) <= 3.4028235e38f ? up : __uint_as_float(0x7fffffffu);
 }
 
-// Eight finished columns d .. d + 7 of a pair: gate, 16 bits.
+// The gate of columns d .. d + 7 of a pair.
+__device__ __forceinline__ void kv8_gate8(const Kv8Args& a, const Kv8Rows& r, uint32_t pair, uint32_t kvh, uint32_t d, uint32_t hd, float4 (&g)[2]) {
+    const uint32_t of = kv8_row_of(a, pair);
+    const float4* from = reinterpret_cast<const float4*>(a.gate + static_cast<size_t>(r.start + of) * a.ldg + (kvh * a.group + pair - of * a.group) * hd + d);
+    g[0] = from[0];
+    g[1] = from[1];
+}
+// Eight finished columns of a pair: gate (where there is one), 16 bits.
 template <typename Act>
-__device__ __forceinline__ void kv8_store8(const Kv8Args& a, const Kv8Rows& r, uint32_t pair, uint32_t kvh, uint32_t d, uint32_t hd, float4 x, float4 y) {
-    const uint32_t of = kv8_row_of(a, pair), row = r.start + of, col = (kvh * a.group + pair - of * a.group) * hd + d;
+__device__ __forceinline__ void kv8_store8(const Kv8Args& a, const Kv8Rows& r, uint32_t pair, uint32_t kvh, uint32_t d, uint32_t hd, float4 x, float4 y, const float4 (&g)[2]) {
+    const uint32_t of = kv8_row_of(a, pair);
     if (a.gate) {
-        const float4 g = *reinterpret_cast<const float4*>(a.gate + static_cast<size_t>(row) * a.ldg + col);
-        const float4 h = *reinterpret_cast<const float4*>(a.gate + static_cast<size_t>(row) * a.ldg + col + 4);
-        x = make_float4(x.x * sigmoid_f(g.x), x.y * sigmoid_f(g.y), x.z * sigmoid_f(g.z), x.w * sigmoid_f(g.w));
-        y = make_float4(y.x * sigmoid_f(h.x), y.y * sigmoid_f(h.y), y.z * sigmoid_f(h.z), y.w * sigmoid_f(h.w));
+        x = make_float4(x.x * sigmoid_f(g[0].x), x.y * sigmoid_f(g[0].y), x.z * sigmoid_f(g[0].z), x.w * sigmoid_f(g[0].w));
+        y = make_float4(y.x * sigmoid_f(g[1].x), y.y * sigmoid_f(g[1].y), y.z * sigmoid_f(g[1].z), y.w * sigmoid_f(g[1].w));
     }
-    *reinterpret_cast<uint4*>(a.y + static_cast<size_t>(row) * a.ldy + col) = make_uint4(Act::pack(x.x, x.y), Act::pack(x.z, x.w), Act::pack(y.x, y.y), Act::pack(y.z, y.w));
+    *reinterpret_cast<uint4*>(a.y + static_cast<size_t>(r.start + of) * a.ldy + (kvh * a.group + pair - of * a.group) * hd + d) =
+        make_uint4(Act::pack(x.x, x.y), Act::pack(x.z, x.w), Act::pack(y.x, y.y), Act::pack(y.z, y.w));
 }
 
 // Columns d .. d + 7 of a pair: sums over the total, then as above. A row that attends nothing has no total: zero.
 template <typename Act>
 __device__ __forceinline__ void kv8_finish(const Kv8Args& a, const Kv8Rows& r, uint32_t pair, uint32_t kvh, uint32_t d, uint32_t hd, float total, float (&o)[8]) {
     const float by = total == 0.f ? 0.f : 1.0f / total;
-    kv8_store8<Act>(a, r, pair, kvh, d, hd, make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by), make_float4(o[4] * by, o[5] * by, o[6] * by, o[7] * by));
+    float4 g[2];
+    if (a.gate) kv8_gate8(a, r, pair, kvh, d, hd, g);
+    kv8_store8<Act>(a, r, pair, kvh, d, hd, make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by), make_float4(o[4] * by, o[5] * by, o[6] * by, o[7] * by), g);
 }
 
 }  // namespace dc

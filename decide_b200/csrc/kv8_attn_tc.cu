@@ -1,9 +1,9 @@
-// dc_kv8_attention for many rows a sequence (heads of 128): the mathematics of kv8_attn.cu on tcgen05.
+// dc_kv8_attention for many rows a sequence: the mathematics of kv8_attn.cu on tcgen05.
 //
-// Products bound it: 4 * 128 operations for each (pair, key), a pair being a (query row, head of the group), against one exponential
+// Products bound it: 4 hd operations for each (pair, key), a pair being a (query row, head of the group), against one exponential
 // and one weight to round. A CTA takes 256 pairs that share a kv head as two tiles of 128, the lanes of tensor memory, which pass the
 // tensor cores back and forth: while one tile's scores are turned into weights, the other's products run.
-//   warps 9..11   codes -> fp16 K and V tiles of 128 keys in shared memory, two stages each. Both lie as rows of keys, 64 columns (128 bytes)
+//   warps 9..11    codes -> fp16 K and V tiles of 128 keys in shared memory, two stages each. Both lie as rows of keys, 64 columns (128 bytes)
 //                 to a swizzled block: K is read as the K-major operand of S = Q K^T, V as the MN-major operand of O += P V, so V needs
 //                 no transposition. The 256 pairs share this work.
 //   warp 8        issues S = Q K^T and O += P V of the two tiles in turn, 64 keys at a time. A tile has two buffers of scores:
@@ -14,7 +14,9 @@
 //                 the maximum of a group and inside the exponential's argument: no instruction per score.
 // Warp 8 shares its scheduler with two softmax warps and nothing else: with a filler there too its issue of products was the bound.
 // The running maximum is lazy as in kv8_attn.cu: O in tensor memory is rescaled only when it grows by more than 2^8.
-// Tensor memory: 2 x (2 x 64 columns of scores + 128 of O). Shared memory: q 64 KB, K and V 64 KB each: one CTA an SM.
+// Tensor memory: 2 x (2 x 64 columns of scores + 128 of O). Shared memory: q 64 KB, K and V 64 KB each: one CTA an SM. Heads of 256 fill
+// both with one tile of 128 pairs (O has 256 columns) and stages of 64 keys; warps 5..7 then help the fillers, who have twice the codes for
+// each product (with three of them a half took 3,500 cycles).
 // Where there are fewer tiles than SMs the keys are cut into chunks, whose results a second kernel joins in chunk order.
 // Every wait is bounded; when one gives up the CTA raises the status word, waits for its products in flight and returns.
 #include "kv8_attn.cuh"
@@ -24,25 +26,34 @@ namespace {
 
 using namespace dc;
 
-constexpr int HD = 128;
-constexpr int kPairs = 256;
-constexpr uint32_t kKeys = 128;      // keys a stage of K or V holds
 constexpr uint32_t kHalf = 64;       // keys a product of scores covers
 constexpr int kThreads = 384;
-constexpr int kFillers = 3;          // warps that turn codes into tiles
-constexpr int kUnits = 11;           // of 32 units of four keys a stage, the first two fillers take 11 each and the last 10
 constexpr uint32_t kTmemCols = 512;
-constexpr int kLd = HD + 4;          // floats of a pair's partial result
+constexpr uint32_t kColO = 256;      // S of tile X, buffer B in columns 128 X + 64 B .., O in 256 + 128 X ..
 constexpr int kScaleSlots = 4;
 
-struct Smem {
-    static constexpr uint32_t kAtom = 128 * 128;            // [128 rows][64 x 16 bit]
-    static constexpr uint32_t kQ = 0;                       // [2 tiles][2 halves of hd]
-    static constexpr uint32_t kK = kQ + 4 * kAtom;          // [2 stages][2 halves]
-    static constexpr uint32_t kV = kK + 4 * kAtom;
-    static constexpr uint32_t kScales = kV + 4 * kAtom;     // float4 [kScaleSlots][8], of 16 keys: K scale, log2 of the V scale, 1 / V scale
-    static constexpr uint32_t kRank = kScales + kScaleSlots * 8 * 16;   // float [256]
-    static constexpr uint32_t kSeen = kRank + kPairs * 4;   // u32 [256]
+template <int HD_>
+struct Shape {
+    static constexpr int HD = HD_;
+    static constexpr int kTiles = 256 / HD;              // tiles of 128 pairs
+    static constexpr int kPairs = 128 * kTiles;
+    static constexpr int kLd = HD + 4;                   // floats of a pair's partial result
+    static constexpr int kHalves = kTiles;               // halves a stage of K or V holds
+    static constexpr uint32_t kKeys = kHalf * kHalves;   // keys of a stage
+    static constexpr int kGroups = kKeys / 16;           // groups of 16 keys
+    // A filler's instruction takes a unit: 512 codes, kRows keys. The 32 units of a stage are shared out evenly, at most kUnits to one.
+    static constexpr uint32_t kRows = 512 / HD;
+    static constexpr int kFillers = HD == 128 ? 3 : 6;
+    static constexpr int kUnits = (32 + kFillers - 1) / kFillers;
+    static constexpr uint32_t kQAtom = 128 * 128;        // [128 pairs][64 x 16 bit]
+    static constexpr uint32_t kAtom = kKeys * 128;       // [keys][64 x 16 bit]
+    static constexpr uint32_t kStage = kAtom * (HD / 64);
+    static constexpr uint32_t kQ = 0;                    // [tiles][HD / 64]
+    static constexpr uint32_t kK = kQ + kTiles * (HD / 64) * kQAtom;   // [2 stages][HD / 64]
+    static constexpr uint32_t kV = kK + 2 * kStage;
+    static constexpr uint32_t kScales = kV + 2 * kStage; // float4 [kScaleSlots][8], of 16 keys: K scale, log2 of the V scale, 1 / V scale
+    static constexpr uint32_t kRank = kScales + kScaleSlots * 8 * 16;   // float [kPairs]
+    static constexpr uint32_t kSeen = kRank + kPairs * 4;   // u32 [kPairs]
     static constexpr uint32_t kBars = kSeen + kPairs * 4;
     static constexpr uint32_t kBytes = kBars + 32 * 8;
 };
@@ -60,11 +71,11 @@ struct Ring {
     }
 };
 
-// V's descriptor: MN-major, 128-byte swizzle. Keys are rows of 128 bytes in groups of 8 (1024 bytes); the two halves of hd lie an atom apart.
-__device__ __forceinline__ uint64_t desc_mn128(uint32_t smem_addr) {
+// V's descriptor: MN-major, 128-byte swizzle. Keys are rows of 128 bytes in groups of 8 (1024 bytes); 64 columns of hd and the next lie `atom` bytes apart.
+__device__ __forceinline__ uint64_t desc_mn128(uint32_t smem_addr, uint32_t atom) {
     uint64_t d = 0;
     d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(Smem::kAtom >> 4) << 16;   // leading byte offset: from 64 columns to the next 64
+    d |= static_cast<uint64_t>(atom >> 4) << 16;   // leading byte offset: from 64 columns to the next 64
     d |= static_cast<uint64_t>(1024 >> 4) << 32;          // stride byte offset: from 8 keys to the next 8
     d |= static_cast<uint64_t>(1) << 46;
     d |= static_cast<uint64_t>(2) << 61;
@@ -73,7 +84,7 @@ __device__ __forceinline__ uint64_t desc_mn128(uint32_t smem_addr) {
 
 // 64 keys of a warp's 32 pairs: scores out of tensor memory, their maximum, then the weights into the columns that the scores came from.
 // MASKED: some pair of the warp does not see all 64 keys; `vis` of them it does. settled(): O may be rescaled.
-template <bool MASKED, typename F>
+template <int HD, bool MASKED, typename F>
 __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, const float4* sc, float mul, int vis, bool scale_o, float& m, float& l, F settled) {
     uint32_t s[2][32];
     tmem_ld_32x32(col_s, s[0]);
@@ -104,7 +115,7 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
         if (scale_o) {
             if (!settled()) return false;
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
+            for (int c = 0; c < HD / 16; ++c) {
                 uint32_t v[16];
                 tmem_ld_32x32_x16(col_o + 16 * c, v);
                 tmem_ld_wait();
@@ -141,10 +152,13 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
     return true;
 }
 
-template <typename Act>
+template <typename Act, int HD>
 __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args a) {
+    using S = Shape<HD>;
+    constexpr int kPairs = S::kPairs, kLd = S::kLd;
+    constexpr uint32_t kKeys = S::kKeys;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     uint64_t* k_full = bars;            // [2] the fillers have written K
     uint64_t* v_full = bars + 2;        // [2]
     uint64_t* k_free = bars + 4;        // [2] both tiles' score products are done
@@ -155,14 +169,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     uint64_t* scale_full = bars + 18;   // [kScaleSlots]
     uint64_t* q_full = bars + 22;       // warps 0..7 have written q
     uint64_t* drain_bar = bars + 23;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+    uint64_t* o_full = bars + 24;       // [2] the tile's last product is done
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     volatile uint32_t* never_flag = tmem_slot + 2;
-    float4* scales = reinterpret_cast<float4*>(smem + Smem::kScales);
-    float* rank = reinterpret_cast<float*>(smem + Smem::kRank);
-    uint32_t* seen = reinterpret_cast<uint32_t*>(smem + Smem::kSeen);
+    float4* scales = reinterpret_cast<float4*>(smem + S::kScales);
+    float* rank = reinterpret_cast<float*>(smem + S::kRank);
+    uint32_t* seen = reinterpret_cast<uint32_t*>(smem + S::kSeen);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join may take its place
     uint32_t id = blockIdx.x;
     const uint32_t z = id % a.chunks;
     id /= a.chunks;
@@ -183,15 +199,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         return;
     }
     const uint32_t here = min(static_cast<uint32_t>(kPairs), pairs - pair0);
-    const bool two = here > 128;   // the second tile has rows
+    const bool two = S::kTiles == 2 && here > 128;   // the second tile has rows
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], kFillers);
-            mbar_init(&v_full[i], kFillers);
+            mbar_init(&k_full[i], S::kFillers);
+            mbar_init(&v_full[i], S::kFillers);
             mbar_init(&k_free[i], 1);
             mbar_init(&v_free[i], 1);
             mbar_init(&pv_done[i], 1);
+            mbar_init(&o_full[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
@@ -228,29 +245,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     const bool whole = most <= a.chunk;
     const bool idle = z && key0 >= most;             // nothing of this tile in this chunk
     const uint32_t key1 = min(most, key0 + a.chunk);
-    const uint32_t halves = idle ? 0u : (key1 - key0 + kHalf - 1) / kHalf, steps = (halves + 1) / 2;
+    const uint32_t halves = idle ? 0u : (key1 - key0 + kHalf - 1) / kHalf, steps = (halves + S::kHalves - 1) / S::kHalves;
     const uint32_t tmem = *tmem_slot;                // 0: all of it is ours
-    constexpr uint32_t kColO = 256;                  // S of tile X, buffer B in columns 128 X + 64 B .., O in 256 + 128 X ..
 
-    if (warp > 8) {
+    if (warp > 8 || (HD == 256 && warp > 4 && warp < 8)) {
         // -------------------------------------------------------------------------------- codes -> fp16 tiles
-        const int w = warp - 9, unit0 = w * kUnits, units = w == kFillers - 1 ? 32 - unit0 : kUnits;   // units of four keys
-        const uint32_t token = static_cast<uint32_t>(a.c.token_stride), four = 4 * token;
+        constexpr int kUnits = S::kUnits;
+        constexpr uint32_t kRows = S::kRows, kPerGroup = 16 / kRows;   // keys of a unit, units of a group of 16 keys
+        const int w = HD == 128 || warp < 8 ? (HD == 128 ? warp - 9 : warp - 5) : warp - 6, unit0 = 32 * w / S::kFillers, units = 32 * (w + 1) / S::kFillers - unit0;
+        const uint32_t token = static_cast<uint32_t>(a.c.token_stride), unit_step = kRows * token;
         const uint32_t* table = a.c.table + static_cast<size_t>(j) * a.c.max_pages;
-        // A lane's place in a unit of four rows of 128 codes: row bits from lane bits 2 and 4, 16-code piece c from bits 0, 1 and 3, so that the
+        // A lane's place in a unit: row bits from lane bits 2 and (of four rows) 4, 16-code piece c from bits 0, 1 and the others, so that the
         // eight lanes of a store's phase, four pieces of two rows, meet all 32 banks of the swizzled tile.
-        const uint32_t fr = ((lane >> 2) & 1) | ((lane >> 4) << 1), c = (lane & 3) | ((lane >> 1) & 4);
+        const uint32_t fr = HD == 128 ? ((lane >> 2) & 1) | ((lane >> 4) << 1) : (lane >> 2) & 1;
+        const uint32_t c = HD == 128 ? (lane & 3) | ((lane >> 1) & 4) : (lane & 3) | ((lane >> 3) << 2);
         const uint8_t* kc = static_cast<const uint8_t*>(a.c.k) + kvh * a.c.head_stride + fr * token + 16 * c;
         const int64_t to_v = static_cast<const uint8_t*>(a.c.v) - static_cast<const uint8_t*>(a.c.k);
         // The filler's units lie in up to kGroups groups of 16 keys, whose pages every lane looks up for itself, a step ahead of the codes.
-        constexpr int kGroups = 4;
-        const uint32_t group0 = unit0 >> 2;
+        constexpr int kGroups = HD == 128 ? 4 : 2;
+        const uint32_t group0 = unit0 / kPerGroup;
         uint32_t page[kGroups];
         auto look_up = [&](uint32_t step) {
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
                 const uint32_t key = key0 + step * kKeys + 16 * (group0 + g);
-                page[g] = key < key1 && group0 + g < 8 ? __ldg(table + (key >> a.page_shift)) : 0u;
+                page[g] = key < key1 && group0 + g < S::kGroups ? __ldg(table + (key >> a.page_shift)) : 0u;
             }
         };
         const uint8_t* at[kGroups];   // first code of the group in K, this lane's; V lies at the same distance from its first
@@ -266,23 +285,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             }
         };
         uint4 kx[kUnits], vx[kUnits];
-        auto load = [&](uint4 (&x)[kUnits], int64_t from, uint32_t step) {   // rows 4 (unit0 + i) + fr; zeros past the last token
-            const uint32_t first = key0 + step * kKeys + 4 * unit0 + fr;
+        auto load = [&](uint4 (&x)[kUnits], int64_t from, uint32_t step) {   // rows kRows (unit0 + i) + fr; zeros past the last token
+            const uint32_t first = key0 + step * kKeys + kRows * unit0 + fr;
             const bool inside = key0 + (step + 1) * kKeys <= key1;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                if (i == kUnits - 1 && units < kUnits) break;
-                const uint32_t u = (unit0 & 3) + i;   // from the start of the first group
-                const uint8_t* group = u < 4 ? at[0] : u < 8 ? at[1] : u < 12 ? at[2] : at[3];
-                if (inside || first + 4 * i < key1) x[i] = __ldg(reinterpret_cast<const uint4*>(group + from + (u & 3) * four));
+                if (i >= 32 / S::kFillers && i >= units) break;
+                const uint32_t u = unit0 % kPerGroup + i;   // from the start of the first group
+                const uint8_t* group = at[0];
+#pragma unroll
+                for (int g = 1; g < kGroups; ++g) group = u < g * kPerGroup ? group : at[g];
+                if (inside || first + kRows * i < key1) x[i] = __ldg(reinterpret_cast<const uint4*>(group + from + (u % kPerGroup) * unit_step));
                 else x[i] = make_uint4(0, 0, 0, 0);
             }
         };
-        // filler 0 also keeps the scales of the stage's eight groups, lane g those of group g
+        // filler 0 also keeps the scales of the stage's groups, lane g those of group g
         uint32_t scale_page = 0;
         float k_scale = 0.f, v_scale = 1.f;
         auto scale_look_up = [&](uint32_t step) {
-            const uint32_t key = key0 + step * kKeys + 16 * (lane & 7);
+            const uint32_t key = key0 + step * kKeys + 16 * (lane % S::kGroups);
             scale_page = key < key1 ? __ldg(table + (key >> a.page_shift)) : 0u;
         };
         auto scale_load = [&] {
@@ -291,16 +312,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             v_scale = a.c.v_scale[s];
             if (scale_page >= a.c.n_pages) k_scale = __uint_as_float(0x7fffffffu);   // what attends it is NaN
         };
-        // 16 codes become the 16-byte pieces 2 c and 2 c + 1 of half c / 4 of the row, at piece ^ (row % 8): with row = 4 u + fr that is one
-        // address, its neighbour at ^ 16, and both at ^ 64 for odd u
-        const uint32_t to0 = (smem_u32(smem) + (c >> 2) * Smem::kAtom + (4 * unit0 + fr) * 128 + (((2 * c) ^ fr) & 7) * 16) ^ ((unit0 & 1) * 64);
+        // 16 codes become the 16-byte pieces 2 c and 2 c + 1 of the row, eight pieces to an atom, at piece ^ (row % 8): with row = kRows u + fr that
+        // is one address and its neighbour at ^ 16, both at ^ 16 (kRows u % 8)
+        const uint32_t to0 = smem_u32(smem) + (c >> 2) * S::kAtom + (kRows * unit0 + fr) * 128 + (((2 * c) ^ fr) & 7) * 16;
         auto store = [&](const uint4 (&x)[kUnits], uint32_t tile) {
-            const uint32_t to = to0 + tile, next = to ^ 64;
+            const uint32_t to = to0 + tile;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                if (i == kUnits - 1 && units < kUnits) break;
-                sts16((i & 1 ? next : to) + 512 * i, low_codes(x[i].x), high_codes(x[i].x), low_codes(x[i].y), high_codes(x[i].y));
-                sts16((i & 1 ? next ^ 16 : to ^ 16) + 512 * i, low_codes(x[i].z), high_codes(x[i].z), low_codes(x[i].w), high_codes(x[i].w));
+                if (i >= 32 / S::kFillers && i >= units) break;
+                const uint32_t swizzle = 16 * (kRows * (unit0 + i) & 7), at_unit = (to ^ swizzle) + kRows * 128 * i, beside = (to ^ swizzle ^ 16) + kRows * 128 * i;
+                sts16(at_unit, low_codes(x[i].x), high_codes(x[i].x), low_codes(x[i].y), high_codes(x[i].y));
+                sts16(beside, low_codes(x[i].z), high_codes(x[i].z), low_codes(x[i].w), high_codes(x[i].w));
             }
         };
         Ring ring;
@@ -318,11 +340,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         }
         for (uint32_t i = 0; i < steps; ++i) {
             if (i >= 2 && !mbar_wait(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81)) break;
-            if (w == 0 && lane < 8) {
+            if (w == 0 && lane < S::kGroups) {
                 const float e = kv8_log2i(v_scale);   // a NaN reaches the total through the weights, not through 1 / V scale
                 scales[(i % kScaleSlots) * 8 + lane] = make_float4(k_scale, e, isnan(e) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(e)))), 0.f);
             }
-            store(kx, Smem::kK + ring.stage * 2 * Smem::kAtom);
+            store(kx, S::kK + ring.stage * S::kStage);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -335,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                 load(kx, 0, i + 1);
             }
             if (i >= 2 && !mbar_wait(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82)) break;
-            store(vx, Smem::kV + ring.stage * 2 * Smem::kAtom);
+            store(vx, S::kV + ring.stage * S::kStage);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[ring.stage]);
@@ -356,49 +378,56 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         // With addresses worked out at run time an MMA took 60 to 70 cycles to issue, more than it takes to run.
         if (steps) {
             constexpr uint32_t idesc_s = umma_idesc(0, 0, 128, kHalf), idesc_o = umma_idesc(0, 0, 128, HD) | (1u << 16);   // B of the V product is MN-major
-            constexpr uint64_t kAtomStep = Smem::kAtom >> 4, kHalfStep = kHalf * 128 >> 4;   // 64 keys: 64 rows of 128 bytes
-            const uint64_t dq = umma_desc_k128(smem_u32(smem) + Smem::kQ), dk = umma_desc_k128(smem_u32(smem) + Smem::kK), dv = desc_mn128(smem_u32(smem) + Smem::kV);
+            constexpr uint64_t kQStep = S::kQAtom >> 4, kStep = S::kAtom >> 4, kStageStep = S::kStage >> 4, kHalfStep = kHalf * 128 >> 4;   // 64 keys: 64 rows of 128 bytes
+            constexpr int kShift = S::kHalves - 1;   // half h lies in stage (h >> kShift) & 1
+            const uint64_t dq = umma_desc_k128(smem_u32(smem) + S::kQ), dk = umma_desc_k128(smem_u32(smem) + S::kK), dv = desc_mn128(smem_u32(smem) + S::kV, S::kAtom);
             const uint32_t n = halves;
             const bool both = two;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
                 const bool done = mbar_wait(bar, parity, abort_flag, a.status, code);
                 return __all_sync(0xffffffffu, done);
             };
-            // half u of a round of four: stage u / 2, buffer u % 2; `last`: the stage's last product of the kind
+            // half u of a round of four: buffer u % 2; `last`: the stage's last product of the kind
             auto scores = [&](int x, int u, bool last) {
+                const int stage = u >> kShift & 1, part = S::kHalves == 2 ? u & 1 : 0;
                 if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint64_t off = (ks >> 2) * kAtomStep + 2 * (ks & 3);
-                        const uint64_t da = dq + (x * 2 * kAtomStep + off), db = dk + ((u >> 1 & 1) * 2 * kAtomStep + (u & 1) * kHalfStep + off);
+                    for (int ks = 0; ks < HD / 16; ++ks) {
+                        const uint64_t da = dq + (x * (HD / 64) + (ks >> 2)) * kQStep + 2 * (ks & 3);
+                        const uint64_t db = dk + (stage * kStageStep + part * kHalfStep + (ks >> 2) * kStep + 2 * (ks & 3));
                         if (ks == 0) umma_bf16_ss<false>(128 * x + 64 * (u & 1), da, db, idesc_s);
                         else umma_bf16_ss<true>(128 * x + 64 * (u & 1), da, db, idesc_s);
                     }
                     umma_commit(&s_full[2 * x + (u & 1)]);
-                    if (last) umma_commit(&k_free[u >> 1 & 1]);
+                    if (last) umma_commit(&k_free[stage]);
                 }
                 __syncwarp();
             };
-            auto values = [&](int x, int u, bool first, bool last) {
+            auto values = [&](int x, int u, bool first, bool last, bool over) {
+                const int stage = u >> kShift & 1, part = S::kHalves == 2 ? u & 1 : 0;
                 if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {   // 16 keys: 8 columns of weights, 2048 bytes of V
-                        const uint64_t db = dv + ((u >> 1 & 1) * 2 * kAtomStep + (u & 1) * kHalfStep + ks * (2048 >> 4));
+                        const uint64_t db = dv + (stage * kStageStep + part * kHalfStep + ks * (2048 >> 4));
                         if (ks == 0 && first) umma_bf16_ts<false>(kColO + 128 * x, 128 * x + 64 * (u & 1) + 8 * ks, db, idesc_o);
                         else umma_bf16_ts<true>(kColO + 128 * x, 128 * x + 64 * (u & 1) + 8 * ks, db, idesc_o);
                     }
                     umma_commit(&pv_done[x]);
-                    if (last) umma_commit(&v_free[u >> 1 & 1]);
+                    if (last) umma_commit(&v_free[stage]);
+                    if (over) umma_commit(&o_full[x]);
                 }
                 __syncwarp();
             };
+            constexpr bool kOwn = S::kHalves == 1;   // every half is a stage of its own
             bool ok = wait(q_full, 0u, 83) && wait(&k_full[0], 0u, 83);
             if (ok) {
                 tc_fence_after_sync();
-                scores(0, 0, !both && n == 1);
+                scores(0, 0, kOwn || (!both && n == 1));
                 if (both) scores(1, 0, n == 1);
                 if (n > 1) {
-                    scores(0, 1, !both);
+                    if (kOwn) ok = wait(&k_full[1], 0u, 83);
+                    if (kOwn) tc_fence_after_sync();
+                    if (ok) scores(0, 1, !both);
                     if (both) scores(1, 1, true);
                 }
             }
@@ -410,16 +439,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                     const uint32_t h = h0 + u;
                     if (!ok || h >= n) break;
                     if (!(ok = wait(&p_full[u & 1], u >> 1, 84))) break;
-                    if (!(u & 1) && !(ok = wait(&v_full[u >> 1], phase, 85))) break;
+                    if ((kOwn || !(u & 1)) && !(ok = wait(&v_full[u >> kShift & 1], kOwn ? u >> 1 : phase, 85))) break;
                     tc_fence_after_sync();
-                    const bool more = h + 2 < n, ends = (u & 1) || h + 1 == n, next_ends = (u & 1) || h + 3 == n;
-                    values(0, u, u == 0 && h0 == 0, !both && ends);
+                    const bool more = h + 2 < n, ends = kOwn || (u & 1) || h + 1 == n, next_ends = kOwn || (u & 1) || h + 3 == n;
+                    values(0, u, u == 0 && h0 == 0, !both && ends, h + 1 == n);
                     if (both && !(ok = wait(&p_full[2 + (u & 1)], u >> 1, 84))) break;
-                    if (more && !(u & 1) && !(ok = wait(&k_full[u >> 1 ^ 1], u ? phase ^ 1u : phase, 86))) break;
+                    if (more && (kOwn || !(u & 1)) && !(ok = wait(&k_full[(u + 2) >> kShift & 1], kOwn ? (u >> 1) ^ 1 : (u ? phase ^ 1u : phase), 86))) break;
                     tc_fence_after_sync();
                     if (more) scores(0, u + 2, !both && next_ends);
                     if (both) {
-                        values(1, u, u == 0 && h0 == 0, ends);
+                        values(1, u, u == 0 && h0 == 0, ends, h + 1 == n);
                         if (more) scores(1, u + 2, next_ends);
                     }
                 }
@@ -436,25 +465,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16), col_o = lanes + kColO + 128 * x;
         bool ok = x == 0 || two;
         if (ok && halves) {
-            // q of the warp's 32 pairs: 8 bytes a lane and row, 16 rows on their way together; bf16 rows are brought into fp16's range as in kv8_attn.cu
+            // q of the warp's 32 pairs: 16 bytes a lane, eight instructions' rows on their way together; bf16 rows are brought into
+            // fp16's range as in kv8_attn.cu. The loops here and at the end are rolled: code that runs once costs its way from memory.
+            constexpr uint32_t kLanes = HD / 8, kAtOnce = 32 / kLanes;   // lanes of a row, rows of an instruction
+            const uint32_t piece = lane % kLanes;
+            uint8_t* to = smem + S::kQ + (x * (HD / 64) + (piece >> 3)) * S::kQAtom;
 #pragma unroll 1
-            for (uint32_t p0 = 32 * warp; p0 < 32 * warp + 32; p0 += 16) {
-                uint2 v[16];
+            for (uint32_t p0 = 32 * warp + lane / kLanes; p0 < 32 * warp + 32; p0 += 8 * kAtOnce) {
+                uint4 v[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t pair = pair0 + p0 + i, of = kv8_row_of(a, pair), row = r.start + of, h = kvh * a.group + pair - of * a.group;
-                    v[i] = p0 + i < here ? *reinterpret_cast<const uint2*>(a.q + static_cast<size_t>(row) * a.ldq + static_cast<size_t>(h) * HD + 4 * lane) : make_uint2(0, 0);
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t pair = pair0 + p0 + kAtOnce * i, of = kv8_row_of(a, pair), h = kvh * a.group + pair - of * a.group;
+                    v[i] = p0 + kAtOnce * i < here ? *reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(r.start + of) * a.ldq + static_cast<size_t>(h) * HD + 8 * piece) : make_uint4(0, 0, 0, 0);
                 }
-                uint32_t top[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top[i] = kv8_query_top<1>(&v[i]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t row = (p0 + i) & 127;
-                    const float up = kv8_query_row<Act, 1>(&v[i], top[i]);
-                    if (lane == 0) rank[p0 + i] = up;
-                    // columns 4 lane ..: half lane / 16, 16-byte piece (lane / 2) % 8, swizzled by the row
-                    *reinterpret_cast<uint2*>(smem + Smem::kQ + (x * 2 + (lane >> 4)) * Smem::kAtom + row * 128 + ((((lane >> 1) & 7) ^ (row & 7)) << 4) + (lane & 1) * 8) = v[i];
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t row = (p0 + kAtOnce * i) & 127;
+                    uint2 w[2] = {make_uint2(v[i].x, v[i].y), make_uint2(v[i].z, v[i].w)};
+                    const float up = kv8_query_row<Act, 2>(w, kv8_query_top<2>(w, kLanes));
+                    if (piece == 0) rank[p0 + kAtOnce * i] = up;
+                    // 16-byte piece of the row, swizzled by the row
+                    *reinterpret_cast<uint4*>(to + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
                 }
             }
             fence_proxy_async_smem();
@@ -466,21 +497,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         const uint32_t see = on ? seen[p] : most;    // pairs past the last are computed (their q is zero) and not stored
         float m = kKv8None, l = 0.f;
         for (uint32_t h = 0; ok && h < halves; ++h) {
-            if (!(ok = mbar_wait(&scale_full[(h >> 1) % kScaleSlots], (h >> 1) / kScaleSlots & 1u, abort_flag, a.status, 88))) break;
+            const uint32_t step = h / S::kHalves;
+            if (!(ok = mbar_wait(&scale_full[step % kScaleSlots], step / kScaleSlots & 1u, abort_flag, a.status, 88))) break;
             if (!(ok = mbar_wait(&s_full[2 * x + (h & 1)], h >> 1 & 1, abort_flag, a.status, 89))) break;
             __syncwarp();
             tc_fence_after_sync();
-            const float4* sc = scales + (h >> 1) % kScaleSlots * 8 + 4 * (h & 1);
+            const float4* sc = scales + step % kScaleSlots * 8 + 4 * (h % S::kHalves);
             const uint32_t key = key0 + h * kHalf, col_s = lanes + 128 * x + 64 * (h & 1);
             const int vis = static_cast<int>(min(see, key + kHalf)) - static_cast<int>(min(see, key));   // of the 64 keys
-            auto settled = [&] {   // the V product of the last 64 keys (the one before it came before these scores)
+            auto settled = [&] {   // the V product of the last 64 keys: the one before it came before these scores, the next has no weights yet
                 const bool done = mbar_wait(&pv_done[x], (h - 1) & 1u, abort_flag, a.status, 91);
                 __syncwarp();
                 tc_fence_after_sync();
                 return done;
             };
-            if (__any_sync(0xffffffffu, vis < static_cast<int>(kHalf))) ok = softmax_half<true>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
-            else ok = softmax_half<false>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
+            if (__any_sync(0xffffffffu, vis < static_cast<int>(kHalf))) ok = softmax_half<HD, true>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
+            else ok = softmax_half<HD, false>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
             if (!ok) break;
             tmem_st_wait();
             tc_fence_before_sync();
@@ -490,22 +522,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         if (ok && runs && !idle) {
             // A tile's q is free once its last product is done (its scores came before it): a warp's 32 rows go through 8 KB of it, 64 columns
             // at a time, so that rows leave in whole pieces. Row r keeps its 16-byte pieces at piece ^ (r % 16).
-            // The last two V products, one after the other: the one before them is done (the last scores came after it), and a wait may
-            // not look further ahead than one phase.
-            bool there = halves < 2 || mbar_wait(&pv_done[x], (halves - 2) & 1u, abort_flag, a.status, 90);
-            if (there && halves) there = mbar_wait(&pv_done[x], (halves - 1) & 1u, abort_flag, a.status, 90);
+            // (pv_done cannot tell: it may have run two phases ahead, and a wait for a phase that lies two back waits for the next one like it)
+            const bool there = halves == 0 || mbar_wait(&o_full[x], 0u, abort_flag, a.status, 90);
             if (there) {
                 __syncwarp();
                 tc_fence_after_sync();
-                uint8_t* stage = smem + Smem::kQ + warp * 8192;
+                uint8_t* stage = smem + S::kQ + warp * 8192;
                 const float by = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
                 const uint32_t first = 32 * warp, col8 = lane & 7;           // pair of the CTA that lane 0 holds; eight lanes a row
                 float* parts = a.part + (static_cast<size_t>(tile_id) * a.chunks + z) * kPairs * kLd;
                 if (!whole && on) *reinterpret_cast<float2*>(parts + p * kLd + HD) = make_float2(m, l);
 #pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    __syncwarp();
+                for (int c = 0; c < HD / 64; ++c) {
+                    // the gates of the eight rows that this lane will store are asked for first (asked for row by row they took 24 us of a tile)
+                    float4 gate[8][2];
+                    if (whole && a.gate) {
 #pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t pr = first + 4 * i + (lane >> 3);
+                            if (pr < here) kv8_gate8(a, r, pair0 + pr, kvh, 64 * c + 8 * col8, HD, gate[i]);
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll 1
                     for (int q4 = 0; q4 < 4; ++q4) {
                         uint32_t v[16];
                         if (halves) {
@@ -523,15 +562,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {                       // four rows at a time
-                        const uint32_t rr = 4 * i + (lane >> 3), pr = first + rr, d = 64 * c + 8 * col8;
-                        const float4 o0 = *reinterpret_cast<const float4*>(stage + rr * 256 + (((2 * col8) ^ (rr & 15)) << 4));
-                        const float4 o1 = *reinterpret_cast<const float4*>(stage + rr * 256 + (((2 * col8 + 1) ^ (rr & 15)) << 4));
+                        const uint32_t rr = 4 * i + (lane >> 3), pr = first + rr;
+                        // 16 bytes of output are 8 columns, side by side; 16 bytes of a partial result are 4: a lane's two pieces lie apart, so
+                        // that the lanes of a row fill whole sectors
+                        const uint32_t p0 = whole ? 2 * col8 : col8, p1 = whole ? p0 + 1 : p0 + 8;
+                        const float4 o0 = *reinterpret_cast<const float4*>(stage + rr * 256 + ((p0 ^ (rr & 15)) << 4));
+                        const float4 o1 = *reinterpret_cast<const float4*>(stage + rr * 256 + ((p1 ^ (rr & 15)) << 4));
                         if (pr >= here) continue;
                         if (whole) {
-                            kv8_store8<Act>(a, r, pair0 + pr, kvh, d, HD, o0, o1);
+                            kv8_store8<Act>(a, r, pair0 + pr, kvh, 64 * c + 8 * col8, HD, o0, o1, gate[i]);
                         } else {
-                            *reinterpret_cast<float4*>(parts + pr * kLd + d) = o0;
-                            *reinterpret_cast<float4*>(parts + pr * kLd + d + 4) = o1;
+                            *reinterpret_cast<float4*>(parts + pr * kLd + 64 * c + 4 * p0) = o0;
+                            *reinterpret_cast<float4*>(parts + pr * kLd + 64 * c + 4 * p1) = o1;
                         }
                     }
                 }
@@ -549,10 +591,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     }
 }
 
-// Joins the chunks of 16 pairs of a tile, in chunk order; a thread takes 8 columns of a pair. Tiles that one chunk held are done already.
-template <typename Act>
+// Joins the chunks of some pairs of a tile, in chunk order; a thread takes 8 columns of a pair. Tiles that one chunk held are done already.
+template <typename Act, int HD>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Args a) {
-    const uint32_t tile_id = blockIdx.x / (kPairs / 16), p = blockIdx.x % (kPairs / 16) * 16 + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+    constexpr int kPairs = Shape<HD>::kPairs, kLd = Shape<HD>::kLd, kCols = HD / 8, kHere = 256 / kCols;   // threads of a pair, pairs of a CTA
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the tiles were still at work
+    const uint32_t tile_id = blockIdx.x / (kPairs / kHere), p = blockIdx.x % (kPairs / kHere) * kHere + threadIdx.x / kCols, d = threadIdx.x % kCols * 8;
     const uint32_t kvh = tile_id % a.c.nkv, mt = a.tiles - 1 - tile_id / a.c.nkv % a.tiles, j = tile_id / a.c.nkv / a.tiles;
     const Kv8Rows r = kv8_rows(a.c, a.q_start, j, a.rows, a.max_q);
     if (!r.ok || r.len > a.max_len) return;
@@ -592,38 +636,56 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Args a) {
 int dc_kv8_attention_tc_warm(dc_ctx* ctx) {
     static bool set[16] = {};
     if (set[ctx->device & 15]) return DC_OK;
-    cudaError_t e = cudaFuncSetAttribute(kv8_attn_tc_kernel<ActF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Smem::kBytes));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv8_attn_tc_kernel<ActBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Smem::kBytes));
-    if (e != cudaSuccess) return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention: cannot opt in to %u bytes of shared memory: %s", Smem::kBytes, cudaGetErrorString(e));
+    typedef void (*fn)(const Kv8Args);
+    const fn all[4] = {kv8_attn_tc_kernel<ActF16, 128>, kv8_attn_tc_kernel<ActBF16, 128>, kv8_attn_tc_kernel<ActF16, 256>, kv8_attn_tc_kernel<ActBF16, 256>};
+    for (int i = 0; i < 4; ++i) {
+        const int bytes = static_cast<int>(i < 2 ? Shape<128>::kBytes : Shape<256>::kBytes);
+        const cudaError_t e = cudaFuncSetAttribute(all[i], cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention: cannot opt in to %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    }
     set[ctx->device & 15] = true;
     return DC_OK;
 }
 
-// How a call is cut: tiles of 256 pairs; where there are fewer of them than SMs, the keys in chunks of at least two steps.
+// How a call is cut: tiles of 256 pairs (heads of 256: 128); where there are fewer of them than SMs, the keys in chunks of at least 256.
 Kv8Cut dc_kv8_attention_tc_cut(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
     Kv8Cut t;
-    const uint64_t pairs = static_cast<uint64_t>(max_q) * (nq / c->nkv);
-    t.tiles = static_cast<uint32_t>((pairs + kPairs - 1) / kPairs);
+    const uint64_t pairs = static_cast<uint64_t>(max_q) * (nq / c->nkv), wide = c->hd == 128 ? Shape<128>::kPairs : Shape<256>::kPairs;
+    t.tiles = static_cast<uint32_t>((pairs + wide - 1) / wide);
     const uint64_t whole = static_cast<uint64_t>(c->n_seqs) * c->nkv * t.tiles;
     uint64_t parts = static_cast<uint64_t>(ctx->sm_count) / whole;
-    const uint64_t most = (max_len + 2 * kKeys - 1) / (2 * kKeys);
+    const uint64_t most = (max_len + 255) / 256;
     parts = parts < 1 ? 1 : parts > most ? most : parts;
-    t.chunk = static_cast<uint32_t>(((max_len + parts - 1) / parts + kKeys - 1) / kKeys * kKeys);
+    t.chunk = static_cast<uint32_t>(((max_len + parts - 1) / parts + 127) / 128 * 128);
     t.chunks = (max_len + t.chunk - 1) / t.chunk;
     t.ctas = whole * t.chunks;
-    t.part_bytes = t.chunks > 1 ? t.ctas * kPairs * kLd * sizeof(float) : 0;
+    t.part_bytes = t.chunks > 1 ? t.ctas * wide * (c->hd + 4) * sizeof(float) : 0;
     return t;
 }
 
 int dc_kv8_attention_tc(dc_ctx* ctx, cudaStream_t s, const dc::Kv8Args& a, uint64_t ctas) {
     const int rc = dc_kv8_attention_tc_warm(ctx);
     if (rc != DC_OK) return rc;
-    const bool f16 = ctx->act_dtype == DC_ACT_F16;
-    auto kern = f16 ? kv8_attn_tc_kernel<ActF16> : kv8_attn_tc_kernel<ActBF16>;
-    kern<<<static_cast<uint32_t>(ctas), kThreads, Smem::kBytes, s>>>(a);
+    const bool f16 = ctx->act_dtype == DC_ACT_F16, narrow = a.c.hd == 128;
+    auto kern = narrow ? (f16 ? kv8_attn_tc_kernel<ActF16, 128> : kv8_attn_tc_kernel<ActBF16, 128>) : (f16 ? kv8_attn_tc_kernel<ActF16, 256> : kv8_attn_tc_kernel<ActBF16, 256>);
+    kern<<<static_cast<uint32_t>(ctas), kThreads, narrow ? Shape<128>::kBytes : Shape<256>::kBytes, s>>>(a);
     const int launched = dc_check_launch(ctx, "kv8_attention (tcgen05)");
     if (launched != DC_OK || a.chunks == 1) return launched;
-    auto join = f16 ? kv8_join_kernel<ActF16> : kv8_join_kernel<ActBF16>;
-    join<<<static_cast<uint32_t>(ctas / a.chunks * (kPairs / 16)), 256, 0, s>>>(a);
+    auto join = narrow ? (f16 ? kv8_join_kernel<ActF16, 128> : kv8_join_kernel<ActBF16, 128>) : (f16 ? kv8_join_kernel<ActF16, 256> : kv8_join_kernel<ActBF16, 256>);
+    const uint32_t per_tile = narrow ? Shape<128>::kPairs / 16 : Shape<256>::kPairs / 8;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<uint32_t>(ctas / a.chunks * per_tile));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, join, a);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention (join): launch failed: %s", cudaGetErrorString(e));
+    }
     return dc_check_launch(ctx, "kv8_attention (join)");
 }

@@ -309,6 +309,10 @@ ATTENTION = [
     dict(lens=[1000, 0, 5], counts=[64, 3, 5], nq=3, nkv=1, hd=128, page=32),
     dict(lens=[2600], counts=[65], nq=2, nkv=2, hd=128, page=64, token_major=True),
     dict(lens=[129, 257, 128, 1], counts=[20, 33, 16, 1], nq=16, nkv=1, hd=128, page=128),
+    dict(lens=[129], counts=[129], nq=1, nkv=1, hd=256, page=16),
+    dict(lens=[300, 40, 700], counts=[50, 40, 70], nq=8, nkv=2, hd=256, page=16),
+    dict(lens=[1000, 0, 5], counts=[64, 3, 5], nq=3, nkv=1, hd=256, page=32, token_major=True),
+    dict(lens=[65, 64, 63, 1], counts=[20, 33, 16, 1], nq=16, nkv=1, hd=256, page=128),
 ]
 
 
@@ -336,7 +340,7 @@ def test_attention(k, act, case):
     k.dev.check_status()
 
 
-@pytest.mark.parametrize("lens,counts,hd", [([5000, 2049, 1], [1, 1, 1], 128), ([2500], [6], 128), ([1200, 700], [1, 2], 256), ([3500, 1500, 300], [40, 20, 30], 128)])
+@pytest.mark.parametrize("lens,counts,hd", [([5000, 2049, 1], [1, 1, 1], 128), ([2500], [6], 128), ([1200, 700], [1, 2], 256), ([3500, 1500, 300], [40, 20, 30], 128), ([2100, 900], [40, 33], 256)])
 def test_attention_in_chunks(k, act, lens, counts, hd):
     """Sequences cut over several CTAs, whose parts are joined."""
     p = _filled(k, lens, 1, hd, 64)
