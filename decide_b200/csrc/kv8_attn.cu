@@ -497,11 +497,14 @@ uint32_t longest(const dc_kv8_cache* c, uint32_t max_len) {
     return max_len == 0 || max_len > cap ? cap : max_len;
 }
 
-// Whole tiles of the tensor cores (256 pairs a CTA) against eights: 128 pairs and more of a sequence, half that over long ones. Measured, us,
-// tcgen05 and here: 64 pairs over 2,307 keys 18 and 13, over 16,000 keys 32 and 46; 64 sequences of 64 pairs over 1,200 keys 171
-// and 132; 256 pairs over 2,307 keys 24 and 24, over 16,000 keys 42 and 124; 16 sequences of 256 pairs over 1,500 keys 64 and 150.
+// Whole tiles of the tensor cores (256 pairs a CTA, 128 of heads of 256) against eights: from 64 pairs a sequence and 2^29 products of a
+// weight and a value on. Measured, us, tcgen05 and here, heads of 128: one sequence of 64 pairs (per kv head, of 8) over 2,307 keys 18.5 and 13.9,
+// over 8,000 24.8 and 28.3; of 256 pairs over 600 keys 19.5 and 10.8, over 2,307 22.3 and 25.1; 16 sequences of 64 pairs over 1,000
+// keys 28 and 36; 64 of 24 pairs over 1,200 keys 150 and 67. Heads of 256, 4 kv heads: 64 pairs over 8,000 keys 29.3 and 27.9; 16
+// sequences of 64 pairs over 1,000 keys 29 and 48.
 bool on_tcgen05(const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
-    return static_cast<uint64_t>(max_q) * (nq / c->nkv) >= (max_len < 8192 ? 128 : 64);
+    const double pairs = static_cast<double>(max_q) * (nq / c->nkv);
+    return pairs >= 64 && pairs * c->n_seqs * c->nkv * max_len * c->hd >= 536870912.0;
 }
 
 }  // namespace

@@ -117,13 +117,15 @@ __device__ __forceinline__ void kv8_gate8(const Kv8Args& a, const Kv8Rows& r, ui
     g[0] = from[0];
     g[1] = from[1];
 }
+// (reciprocal and exponential to 2^-21: the output has at most 11 bits)
+__device__ __forceinline__ float kv8_sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 // Eight finished columns of a pair: gate (where there is one), 16 bits.
 template <typename Act>
 __device__ __forceinline__ void kv8_store8(const Kv8Args& a, const Kv8Rows& r, uint32_t pair, uint32_t kvh, uint32_t d, uint32_t hd, float4 x, float4 y, const float4 (&g)[2]) {
     const uint32_t of = kv8_row_of(a, pair);
     if (a.gate) {
-        x = make_float4(x.x * sigmoid_f(g[0].x), x.y * sigmoid_f(g[0].y), x.z * sigmoid_f(g[0].z), x.w * sigmoid_f(g[0].w));
-        y = make_float4(y.x * sigmoid_f(g[1].x), y.y * sigmoid_f(g[1].y), y.z * sigmoid_f(g[1].z), y.w * sigmoid_f(g[1].w));
+        x = make_float4(x.x * kv8_sigmoid(g[0].x), x.y * kv8_sigmoid(g[0].y), x.z * kv8_sigmoid(g[0].z), x.w * kv8_sigmoid(g[0].w));
+        y = make_float4(y.x * kv8_sigmoid(g[1].x), y.y * kv8_sigmoid(g[1].y), y.z * kv8_sigmoid(g[1].z), y.w * kv8_sigmoid(g[1].w));
     }
     *reinterpret_cast<uint4*>(a.y + static_cast<size_t>(r.start + of) * a.ldy + (kvh * a.group + pair - of * a.group) * hd + d) =
         make_uint4(Act::pack(x.x, x.y), Act::pack(x.z, x.w), Act::pack(y.x, y.y), Act::pack(y.z, y.w));

@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     uint64_t* q_full = bars + 22;       // warps 0..7 have written q
     uint64_t* drain_bar = bars + 23;
     uint64_t* o_full = bars + 24;       // [2] the tile's last product is done
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+    uint64_t* l_full = bars + 26;       // heads of 256: the pairs' divisors are there
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     volatile uint32_t* never_flag = tmem_slot + 2;
     float4* scales = reinterpret_cast<float4*>(smem + S::kScales);
@@ -217,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         for (int i = 0; i < kScaleSlots; ++i) mbar_init(&scale_full[i], 1);
         mbar_init(q_full, two ? 8 : 4);
         mbar_init(drain_bar, 1);
+        mbar_init(l_full, 4);
         *abort_flag = 0u;
         *never_flag = 0u;
         fence_mbar_init();
@@ -248,6 +250,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     const uint32_t halves = idle ? 0u : (key1 - key0 + kHalf - 1) / kHalf, steps = (halves + S::kHalves - 1) / S::kHalves;
     const uint32_t tmem = *tmem_slot;                // 0: all of it is ours
 
+    bool ok = true;                                  // this warp has not given up
+    float m = kKv8None, l = 0.f;                     // softmax warps: of their pair
     if (warp > 8 || (HD == 256 && warp > 4 && warp < 8)) {
         // -------------------------------------------------------------------------------- codes -> fp16 tiles
         constexpr int kUnits = S::kUnits;
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             look_up(1);
         }
         for (uint32_t i = 0; i < steps; ++i) {
-            if (i >= 2 && !mbar_wait(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81)) break;
+            if (i >= 2 && !(ok = mbar_wait(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81))) break;
             if (w == 0 && lane < S::kGroups) {
                 const float e = kv8_log2i(v_scale);   // a NaN reaches the total through the weights, not through 1 / V scale
                 scales[(i % kScaleSlots) * 8 + lane] = make_float4(k_scale, e, isnan(e) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(e)))), 0.f);
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                 to_page(i + 1);
                 load(kx, 0, i + 1);
             }
-            if (i >= 2 && !mbar_wait(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82)) break;
+            if (i >= 2 && !(ok = mbar_wait(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82))) break;
             store(vx, S::kV + ring.stage * S::kStage);
             fence_proxy_async_smem();
             __syncwarp();
@@ -419,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                 __syncwarp();
             };
             constexpr bool kOwn = S::kHalves == 1;   // every half is a stage of its own
-            bool ok = wait(q_full, 0u, 83) && wait(&k_full[0], 0u, 83);
+            ok = wait(q_full, 0u, 83) && wait(&k_full[0], 0u, 83);
             if (ok) {
                 tc_fence_after_sync();
                 scores(0, 0, kOwn || (!both && n == 1));
@@ -463,8 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         // -------------------------------------------------------------------------------- softmax: one thread per pair
         const uint32_t x = warp >> 2, p = tid;       // tile; pair of the CTA
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16), col_o = lanes + kColO + 128 * x;
-        bool ok = x == 0 || two;
-        if (ok && halves) {
+        const bool runs = x == 0 || two;
+        if (runs && halves) {
             // q of the warp's 32 pairs: 16 bytes a lane, eight instructions' rows on their way together; bf16 rows are brought into
             // fp16's range as in kv8_attn.cu. The loops here and at the end are rolled: code that runs once costs its way from memory.
             constexpr uint32_t kLanes = HD / 8, kAtOnce = 32 / kLanes;   // lanes of a row, rows of an instruction
@@ -492,11 +496,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        const bool on = p < here, runs = ok;
-        const float mul = ok && halves ? a.scale * rank[p] : 0.f;
+        const bool on = p < here;
+        const float mul = runs && halves ? a.scale * rank[p] : 0.f;
         const uint32_t see = on ? seen[p] : most;    // pairs past the last are computed (their q is zero) and not stored
-        float m = kKv8None, l = 0.f;
-        for (uint32_t h = 0; ok && h < halves; ++h) {
+        for (uint32_t h = 0; runs && ok && h < halves; ++h) {
             const uint32_t step = h / S::kHalves;
             if (!(ok = mbar_wait(&scale_full[step % kScaleSlots], step / kScaleSlots & 1u, abort_flag, a.status, 88))) break;
             if (!(ok = mbar_wait(&s_full[2 * x + (h & 1)], h >> 1 & 1, abort_flag, a.status, 89))) break;
@@ -519,62 +522,74 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[2 * x + (h & 1)]);
         }
-        if (ok && runs && !idle) {
-            // A tile's q is free once its last product is done (its scores came before it): a warp's 32 rows go through 8 KB of it, 64 columns
-            // at a time, so that rows leave in whole pieces. Row r keeps its 16-byte pieces at piece ^ (r % 16).
-            // (pv_done cannot tell: it may have run two phases ahead, and a wait for a phase that lies two back waits for the next one like it)
-            const bool there = halves == 0 || mbar_wait(&o_full[x], 0u, abort_flag, a.status, 90);
-            if (there) {
+        // the divisor, for whoever stores the pair's columns
+        if (HD == 256 && x == 0 && ok && !idle) {
+            rank[p] = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(l_full);
+        }
+    }
+
+    // ------------------------------------------------------------------------------------ output
+    // Warps 0..7, 32 pairs each; of heads of 256, warps 0..3 store columns 0..127 of the tile's pairs and warps 4..7 the others (a warp reaches the
+    // lanes of tensor memory that its number modulo four gives). A tile's q is free once its last product is done (its scores came
+    // before it): rows go through 8 KB of it, 64 columns at a time, so that they leave in whole pieces. Row r keeps its 16-byte pieces at
+    // piece ^ (r % 16).
+    if (warp < 8 && ok && !idle && (HD == 256 || warp < 4 || two)) {
+        const uint32_t x = HD == 256 ? 0 : warp >> 2, part = HD == 256 ? warp >> 2 : 0, first = HD == 256 ? 32 * (warp & 3) : 32 * warp;   // tile, 128 columns, pair of lane 0
+        // (pv_done cannot tell: it may have run two phases ahead, and a wait for a phase that lies two back waits for the next one like it)
+        const bool there = (HD == 128 || mbar_wait(l_full, 0u, abort_flag, a.status, 92)) && (halves == 0 || mbar_wait(&o_full[x], 0u, abort_flag, a.status, 90));
+        if (there) {
+            __syncwarp();
+            tc_fence_after_sync();
+            uint8_t* stage = smem + S::kQ + warp * 8192;
+            const float by = HD == 256 ? rank[first + lane] : whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+            const uint32_t col8 = lane & 7, col_o = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColO + 128 * (x + part);   // eight lanes a row
+            float* parts = a.part + (static_cast<size_t>(tile_id) * a.chunks + z) * kPairs * kLd;
+            if (!whole && part == 0 && first + lane < here) *reinterpret_cast<float2*>(parts + (first + lane) * kLd + HD) = make_float2(m, l);
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t d = 128 * part + 64 * c;
+                // the gates of the eight rows that this lane will store are asked for first (asked for row by row they took 24 us of a tile)
+                float4 gate[8][2];
+                if (whole && a.gate) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t pr = first + 4 * i + (lane >> 3);
+                        if (pr < here) kv8_gate8(a, r, pair0 + pr, kvh, d + 8 * col8, HD, gate[i]);
+                    }
+                }
                 __syncwarp();
-                tc_fence_after_sync();
-                uint8_t* stage = smem + S::kQ + warp * 8192;
-                const float by = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
-                const uint32_t first = 32 * warp, col8 = lane & 7;           // pair of the CTA that lane 0 holds; eight lanes a row
-                float* parts = a.part + (static_cast<size_t>(tile_id) * a.chunks + z) * kPairs * kLd;
-                if (!whole && on) *reinterpret_cast<float2*>(parts + p * kLd + HD) = make_float2(m, l);
 #pragma unroll 1
-                for (int c = 0; c < HD / 64; ++c) {
-                    // the gates of the eight rows that this lane will store are asked for first (asked for row by row they took 24 us of a tile)
-                    float4 gate[8][2];
-                    if (whole && a.gate) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint32_t pr = first + 4 * i + (lane >> 3);
-                            if (pr < here) kv8_gate8(a, r, pair0 + pr, kvh, 64 * c + 8 * col8, HD, gate[i]);
-                        }
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    uint32_t v[16];
+                    if (halves) {
+                        tmem_ld_32x32_x16(col_o + 64 * c + 16 * q4, v);
+                        tmem_ld_wait();
                     }
-                    __syncwarp();
-#pragma unroll 1
-                    for (int q4 = 0; q4 < 4; ++q4) {
-                        uint32_t v[16];
-                        if (halves) {
-                            tmem_ld_32x32_x16(col_o + 64 * c + 16 * q4, v);
-                            tmem_ld_wait();
-                        }
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            uint4 o = make_uint4(0, 0, 0, 0);
-                            if (halves) o = make_uint4(__float_as_uint(__uint_as_float(v[e]) * by), __float_as_uint(__uint_as_float(v[e + 1]) * by),
-                                                       __float_as_uint(__uint_as_float(v[e + 2]) * by), __float_as_uint(__uint_as_float(v[e + 3]) * by));
-                            *reinterpret_cast<uint4*>(stage + lane * 256 + (((4 * q4 + e / 4) ^ (lane & 15)) << 4)) = o;
-                        }
+                    for (int e = 0; e < 16; e += 4) {
+                        uint4 o = make_uint4(0, 0, 0, 0);
+                        if (halves) o = make_uint4(__float_as_uint(__uint_as_float(v[e]) * by), __float_as_uint(__uint_as_float(v[e + 1]) * by),
+                                                   __float_as_uint(__uint_as_float(v[e + 2]) * by), __float_as_uint(__uint_as_float(v[e + 3]) * by));
+                        *reinterpret_cast<uint4*>(stage + lane * 256 + (((4 * q4 + e / 4) ^ (lane & 15)) << 4)) = o;
                     }
-                    __syncwarp();
+                }
+                __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {                       // four rows at a time
-                        const uint32_t rr = 4 * i + (lane >> 3), pr = first + rr;
-                        // 16 bytes of output are 8 columns, side by side; 16 bytes of a partial result are 4: a lane's two pieces lie apart, so
-                        // that the lanes of a row fill whole sectors
-                        const uint32_t p0 = whole ? 2 * col8 : col8, p1 = whole ? p0 + 1 : p0 + 8;
-                        const float4 o0 = *reinterpret_cast<const float4*>(stage + rr * 256 + ((p0 ^ (rr & 15)) << 4));
-                        const float4 o1 = *reinterpret_cast<const float4*>(stage + rr * 256 + ((p1 ^ (rr & 15)) << 4));
-                        if (pr >= here) continue;
-                        if (whole) {
-                            kv8_store8<Act>(a, r, pair0 + pr, kvh, 64 * c + 8 * col8, HD, o0, o1, gate[i]);
-                        } else {
-                            *reinterpret_cast<float4*>(parts + pr * kLd + 64 * c + 4 * p0) = o0;
-                            *reinterpret_cast<float4*>(parts + pr * kLd + 64 * c + 4 * p1) = o1;
-                        }
+                for (int i = 0; i < 8; ++i) {                       // four rows at a time
+                    const uint32_t rr = 4 * i + (lane >> 3), pr = first + rr;
+                    // 16 bytes of output are 8 columns, side by side; 16 bytes of a partial result are 4: a lane's two pieces lie apart, so
+                    // that the lanes of a row fill whole sectors
+                    const uint32_t p0 = whole ? 2 * col8 : col8, p1 = whole ? p0 + 1 : p0 + 8;
+                    const float4 o0 = *reinterpret_cast<const float4*>(stage + rr * 256 + ((p0 ^ (rr & 15)) << 4));
+                    const float4 o1 = *reinterpret_cast<const float4*>(stage + rr * 256 + ((p1 ^ (rr & 15)) << 4));
+                    if (pr >= here) continue;
+                    if (whole) {
+                        kv8_store8<Act>(a, r, pair0 + pr, kvh, d + 8 * col8, HD, o0, o1, gate[i]);
+                    } else {
+                        *reinterpret_cast<float4*>(parts + pr * kLd + d + 4 * p0) = o0;
+                        *reinterpret_cast<float4*>(parts + pr * kLd + d + 4 * p1) = o1;
                     }
                 }
             }

@@ -316,9 +316,14 @@ ATTENTION = [
 ]
 
 
-def _filled(k, lens, nkv, hd, page, token_major=False, size=1.0, seed=0):
+# A table with room for this many tokens a sequence, and no length given, makes 64 and more (row, head) pairs of a kv head a call for whole
+# tiles of the tensor cores, however short the sequences are.
+ROOM = 65536
+
+
+def _filled(k, lens, nkv, hd, page, token_major=False, size=1.0, seed=0, room=0):
     pages = [-(-n // page) for n in lens]
-    p = Pair(k, n_pages=sum(pages) + 2, nkv=nkv, hd=hd, n_seqs=len(lens), max_pages=max(pages) + 1, page=page, token_major=token_major)
+    p = Pair(k, n_pages=sum(pages) + 2, nkv=nkv, hd=hd, n_seqs=len(lens), max_pages=max(max(pages) + 1, room // page), page=page, token_major=token_major)
     step = [n // 2 for n in lens]       # in two steps, so that the sequences' pages interleave
     for part in (step, [n - s for n, s in zip(lens, step)]):
         p.extend(part)
@@ -338,15 +343,23 @@ def test_attention(k, act, case):
     qpos = [kv8.NO_KEYS if n == 0 or rng.rand() < 0.2 else rng.randint(n) for n, m in zip(c["lens"], counts) for _ in range(m)]
     p.attend(counts, nq, qpos=qpos, seed=2, max_len=0)
     k.dev.check_status()
+    if max(counts) * (nq // c["nkv"]) >= 64:
+        p = _filled(k, room=ROOM, **c)
+        p.attend(counts, nq, gate=False, max_len=0)
+        p.attend(counts, nq, gate=True, pad=8, seed=1, max_len=0)
+        p.attend(counts, nq, qpos=qpos, seed=2, max_len=0)
+        k.dev.check_status()
 
 
 @pytest.mark.parametrize("lens,counts,hd", [([5000, 2049, 1], [1, 1, 1], 128), ([2500], [6], 128), ([1200, 700], [1, 2], 256), ([3500, 1500, 300], [40, 20, 30], 128), ([2100, 900], [40, 33], 256)])
 def test_attention_in_chunks(k, act, lens, counts, hd):
     """Sequences cut over several CTAs, whose parts are joined."""
-    p = _filled(k, lens, 1, hd, 64)
-    p.attend(counts, 4)
-    p.attend(counts, 4, qpos=[n // (i + 1) - 1 if n > 1 else 0 for n, m in zip(lens, counts) for i in range(m)], seed=1)
-    k.dev.check_status()
+    for room in (0, ROOM) if max(counts) >= 16 else (0,):
+        p = _filled(k, lens, 1, hd, 64, room=room)
+        max_len = 0 if room else None
+        p.attend(counts, 4, max_len=max_len)
+        p.attend(counts, 4, qpos=[n // (i + 1) - 1 if n > 1 else 0 for n, m in zip(lens, counts) for i in range(m)], seed=1, max_len=max_len)
+        k.dev.check_status()
 
 
 def test_attention_long_sequences_whole(k):
@@ -363,6 +376,28 @@ def test_attention_few_rows_of_many_heads(k, act):
     for hd, counts in ((128, [1, 2]), (128, [1, 5]), (256, [2, 3])):
         p = _filled(k, [70, 300], 2, hd, 32)
         p.attend(counts, 32)
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_attention_repeats_bit_for_bit(k, hd):
+    """The same call many times, with the GPU to itself and behind other calls: the same bits, and no wait that runs out."""
+    p = _filled(k, [129, 257, 128, 1, 900], 1, hd, 128, room=ROOM)
+    counts, nq = [20, 33, 16, 1, 24], 16
+    first = [p.attend(counts, nq, max_len=0), p.attend(counts, nq, seed=1, max_len=400 * 128)]
+    rows, width = sum(counts), nq * hd
+    gen = torch.Generator().manual_seed(100)
+    q = (torch.randn(rows + 2, width, generator=gen) * 1.5).to(k.dev.act_torch).cuda()
+    g = torch.randn(rows + 2, width + 4, generator=gen).cuda()
+    start = p.ints(np.concatenate([[0], np.cumsum(counts)]))
+    y = torch.empty_like(first[0])
+    for i in range(200):
+        y.fill_(SENTINEL)
+        p.ops.attention(None, p.gpu, 0, q, g, start, None, y, rows, width, width + 4, width + 8, nq, max(counts), 0 if i % 2 else 300 * 128)
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        if i % 2:
+            assert torch.equal(y, first[0]), i
     k.dev.check_status()
 
 
