@@ -64,6 +64,7 @@ template <typename Act, int VECS>
 __global__ void __launch_bounds__(kThreads)
 kv8_append_kernel(dc_kv8_cache c, uint32_t page_shift, uint32_t row_shift, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, uint32_t ldk,
                   uint32_t ldv, const uint32_t* __restrict__ row_start, uint32_t rows, uint32_t max_rows, int* __restrict__ status) {
+    kv8_begin();
     const uint32_t j = blockIdx.z, head = blockIdx.y;
     const bool reports = head == 0 && threadIdx.x == 0;
     const uint32_t r0 = row_start[j], r1 = row_start[j + 1], len = c.lens[j];
@@ -130,11 +131,12 @@ kv8_append_kernel(dc_kv8_cache c, uint32_t page_shift, uint32_t row_shift, const
 }
 
 template <typename Act>
-void launch(dim3 grid, cudaStream_t s, uint32_t vecs, const dc_kv8_cache& c, const uint16_t* k, const uint16_t* v, uint32_t ldk, uint32_t ldv,
-            const uint32_t* row_start, uint32_t rows, uint32_t max_rows, int* status) {
+int launch(dc_ctx* ctx, dim3 grid, cudaStream_t s, uint32_t vecs, const dc_kv8_cache& c, const uint16_t* k, const uint16_t* v, uint32_t ldk, uint32_t ldv,
+            const uint32_t* row_start, uint32_t rows, uint32_t max_rows) {
     auto kern = vecs <= 1 ? kv8_append_kernel<Act, 1> : vecs <= 2 ? kv8_append_kernel<Act, 2> : vecs <= 4 ? kv8_append_kernel<Act, 4>
               : vecs <= 8 ? kv8_append_kernel<Act, 8> : kv8_append_kernel<Act, 16>;
-    kern<<<grid, kThreads, 0, s>>>(c, __builtin_ctz(c.page_size), __builtin_ctz(c.hd / 8), k, v, ldk, ldv, row_start, rows, max_rows, status);
+    return dc_kv8_launch(ctx, "kv8_append", kern, false, grid, kThreads, 0, s, c, __builtin_ctz(c.page_size), __builtin_ctz(c.hd / 8), k, v, ldk, ldv, row_start, rows,
+                         max_rows, ctx->status_dev);
 }
 
 }  // namespace
@@ -163,7 +165,6 @@ extern "C" int dc_kv8_append(dc_ctx* ctx, void* stream, const dc_kv8_cache* cach
     const uint32_t fit = most < c.page_size ? most : c.page_size;
     const uint32_t vecs = (fit * (c.hd / 8) + kThreads - 1) / kThreads;
     auto go = ctx->act_dtype == DC_ACT_F16 ? launch<dc::ActF16> : launch<dc::ActBF16>;
-    go(dim3(spans, c.nkv, c.n_seqs), static_cast<cudaStream_t>(stream), vecs, c, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
-       ldk, ldv, row_start, rows, max_rows, ctx->status_dev);
-    return dc_check_launch(ctx, "kv8_append");
+    return go(ctx, dim3(spans, c.nkv, c.n_seqs), static_cast<cudaStream_t>(stream), vecs, c, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+              ldk, ldv, row_start, rows, max_rows);
 }

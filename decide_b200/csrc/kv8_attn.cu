@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     uint32_t* seen = reinterpret_cast<uint32_t*>(smem + S::kSeen);   // tokens that a pair attends
     float* rank = reinterpret_cast<float*>(seen + kPairs);           // power of two that a pair's q was divided by
 
+    kv8_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint32_t id = blockIdx.x;
     const uint32_t z = id % a.chunks;
@@ -581,6 +582,5 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (tc) return dc_kv8_attention_tc(ctx, s, a, t.ctas);
     const Variant v = f16 ? pick<dc::ActF16>(cache->hd, t.nt) : pick<dc::ActBF16>(cache->hd, t.nt);
-    v.f<<<static_cast<uint32_t>(t.ctas), v.threads, v.bytes, s>>>(a);
-    return dc_check_launch(ctx, "kv8_attention");
+    return dc_kv8_launch(ctx, "kv8_attention", v.f, 2 * t.ctas <= static_cast<uint64_t>(ctx->sm_count), dim3(static_cast<uint32_t>(t.ctas)), v.threads, v.bytes, s, a);
 }

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     uint32_t* seen = reinterpret_cast<uint32_t*>(smem + S::kSeen);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join may take its place
+    kv8_begin();
     uint32_t id = blockIdx.x;
     const uint32_t z = id % a.chunks;
     id /= a.chunks;
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
 template <typename Act, int HD>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Args a) {
     constexpr int kPairs = Shape<HD>::kPairs, kLd = Shape<HD>::kLd, kCols = HD / 8, kHere = 256 / kCols;   // threads of a pair, pairs of a CTA
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the tiles were still at work
+    kv8_begin();
     const uint32_t tile_id = blockIdx.x / (kPairs / kHere), p = blockIdx.x % (kPairs / kHere) * kHere + threadIdx.x / kCols, d = threadIdx.x % kCols * 8;
     const uint32_t kvh = tile_id % a.c.nkv, mt = a.tiles - 1 - tile_id / a.c.nkv % a.tiles, j = tile_id / a.c.nkv / a.tiles;
     const Kv8Rows r = kv8_rows(a.c, a.q_start, j, a.rows, a.max_q);
@@ -683,24 +683,9 @@ int dc_kv8_attention_tc(dc_ctx* ctx, cudaStream_t s, const dc::Kv8Args& a, uint6
     if (rc != DC_OK) return rc;
     const bool f16 = ctx->act_dtype == DC_ACT_F16, narrow = a.c.hd == 128;
     auto kern = narrow ? (f16 ? kv8_attn_tc_kernel<ActF16, 128> : kv8_attn_tc_kernel<ActBF16, 128>) : (f16 ? kv8_attn_tc_kernel<ActF16, 256> : kv8_attn_tc_kernel<ActBF16, 256>);
-    kern<<<static_cast<uint32_t>(ctas), kThreads, narrow ? Shape<128>::kBytes : Shape<256>::kBytes, s>>>(a);
-    const int launched = dc_check_launch(ctx, "kv8_attention (tcgen05)");
+    const int launched = dc_kv8_launch(ctx, "kv8_attention (tcgen05)", kern, false, dim3(static_cast<uint32_t>(ctas)), kThreads, narrow ? Shape<128>::kBytes : Shape<256>::kBytes, s, a);
     if (launched != DC_OK || a.chunks == 1) return launched;
     auto join = narrow ? (f16 ? kv8_join_kernel<ActF16, 128> : kv8_join_kernel<ActBF16, 128>) : (f16 ? kv8_join_kernel<ActF16, 256> : kv8_join_kernel<ActBF16, 256>);
     const uint32_t per_tile = narrow ? Shape<128>::kPairs / 16 : Shape<256>::kPairs / 8;
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<uint32_t>(ctas / a.chunks * per_tile));
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, join, a);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention (join): launch failed: %s", cudaGetErrorString(e));
-    }
-    return dc_check_launch(ctx, "kv8_attention (join)");
+    return dc_kv8_launch(ctx, "kv8_attention (join)", join, true, dim3(static_cast<uint32_t>(ctas / a.chunks * per_tile)), 256, 0, s, a);
 }

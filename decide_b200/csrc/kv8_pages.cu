@@ -82,10 +82,6 @@ __device__ uint32_t find_free(const uint32_t* refs, uint32_t n_pages, uint32_t n
 // A sequence's pages, from its length as it is now; flags a length that its row of the table cannot hold.
 __device__ __forceinline__ bool length_fits(const dc_kv8_cache& c, uint32_t len) { return len <= c.max_pages * c.page_size; }
 
-// The copying kernel is launched while the deciding one runs (programmatic dependent launch) and waits for it here.
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_launcher() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // refs of the pages of sequences ids[0 .. n): `by` = -1 gives them up, + 1 takes them back. Warps take the sequences in turn. *bad is set
 // where a page id is outside the pool (it is passed over) or a page that nobody held is given up.
 __device__ __forceinline__ void release(const dc_kv8_cache& c, const uint32_t* ids, uint32_t n, int by, int* bad) {
@@ -105,6 +101,7 @@ extend_kernel(dc_kv8_cache c, const uint32_t* __restrict__ add, Plan plan, int* 
     __shared__ uint32_t sums[64];
     __shared__ int bad;
     uint32_t turn = 0;
+    kv8_begin();
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
     // what each sequence lacks, and how many pages the ones before it in the round lack
@@ -166,7 +163,7 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
     __shared__ int bad;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t turn = 0;
-    launch_dependents();
+    kv8_begin();
     for (uint32_t i = threadIdx.x; i < (c.n_seqs + 31) / 32; i += kPlanThreads) taken[i] = 0u;
     if (threadIdx.x == 0) {
         bad = 0;
@@ -256,6 +253,7 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
 }
 
 __global__ void __launch_bounds__(128) free_kernel(dc_kv8_cache c, const uint32_t* __restrict__ seqs, int* __restrict__ status) {
+    kv8_begin();
     const uint32_t j = seqs[blockIdx.x];
     __shared__ uint32_t claimed;
     if (threadIdx.x == 0) {
@@ -280,7 +278,7 @@ __global__ void __launch_bounds__(128) free_kernel(dc_kv8_cache c, const uint32_
 __global__ void __launch_bounds__(kPlanThreads) compact_kernel(dc_kv8_cache c, Plan plan, uint32_t* __restrict__ live_out) {
     __shared__ uint32_t sums[64];
     uint32_t turn = 0, live = 0, mask = 0;   // of four pages, those in use
-    launch_dependents();
+    kv8_begin();
     auto look = [&](uint32_t at) {
         mask = 0;
 #pragma unroll
@@ -334,7 +332,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(dc_kv8_cache c, P
 // page_size * hd codes and a scale. No page is both read and written (the lists are made so).
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(dc_kv8_cache c, Plan plan, bool rename, int* __restrict__ status) {
     const uint32_t lane = threadIdx.x & 31;
-    wait_for_launcher();
+    kv8_begin();
     const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kCopyThreads / 32);
     const uint64_t units = static_cast<uint64_t>(plan.head[0]) * c.layers * 2 * c.nkv;
     const uint32_t per_row = c.hd / 16, vectors = c.page_size * per_row;
@@ -387,25 +385,6 @@ uint32_t copy_grid(const dc_ctx* ctx, const dc_kv8_cache* c, uint64_t moves) {
     const uint64_t units = moves * c->layers * 2 * c->nkv, ctas = (units + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
     const uint64_t most = static_cast<uint64_t>(ctx->sm_count) * 8;
     return static_cast<uint32_t>(ctas < 1 ? 1 : ctas < most ? ctas : most);
-}
-
-// Launches the copying kernel so that it may start while the deciding one, enqueued just before, still runs.
-int launch_copies(dc_ctx* ctx, cudaStream_t s, const char* what, uint32_t grid, const dc_kv8_cache& c, Plan plan, bool rename) {
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kCopyThreads);
-    cfg.stream = s;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, copy_kernel, c, plan, rename, ctx->status_dev);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return dc_fail(ctx, DC_CUDA_ERROR, "%s: launch failed: %s", what, cudaGetErrorString(e));
-    }
-    return dc_check_launch(ctx, what);
 }
 
 int pages_begin(dc_ctx* ctx, const char* who, const dc_kv8_cache* cache, Plan* plan) {
@@ -474,8 +453,7 @@ extern "C" int dc_kv8_extend(dc_ctx* ctx, void* stream, const dc_kv8_cache* cach
     const dc_device_scope scope(ctx);
     Plan plan;
     if ((rc = pages_begin(ctx, "kv8_extend", cache, &plan)) != DC_OK) return rc;
-    extend_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(*cache, add, plan, ctx->status_dev);
-    return dc_check_launch(ctx, "kv8_extend");
+    return dc_kv8_launch(ctx, "kv8_extend", extend_kernel, true, dim3(1), kPlanThreads, 0, static_cast<cudaStream_t>(stream), *cache, add, plan, ctx->status_dev);
 }
 
 extern "C" int dc_kv8_fork(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, const uint32_t* src, const uint32_t* dst, uint32_t n, uint32_t deep) {
@@ -490,10 +468,11 @@ extern "C" int dc_kv8_fork(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache,
     Plan plan;
     if ((rc = pages_begin(ctx, "kv8_fork", cache, &plan)) != DC_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    fork_kernel<<<1, kPlanThreads, (cache->n_seqs + 31) / 32 * 4, s>>>(*cache, src, dst, n, deep != 0, plan, ctx->status_dev);
-    if ((rc = dc_check_launch(ctx, "kv8_fork")) != DC_OK) return rc;
+    if ((rc = dc_kv8_launch(ctx, "kv8_fork", fork_kernel, true, dim3(1), kPlanThreads, (cache->n_seqs + 31) / 32 * 4, s, *cache, src, dst, n, deep != 0, plan, ctx->status_dev)) != DC_OK)
+        return rc;
     const uint64_t most = deep ? static_cast<uint64_t>(n) * cache->max_pages : n;
-    return launch_copies(ctx, s, "kv8_fork (copies)", copy_grid(ctx, cache, most < cache->n_pages ? most : cache->n_pages), *cache, plan, false);
+    return dc_kv8_launch(ctx, "kv8_fork (copies)", copy_kernel, true, dim3(copy_grid(ctx, cache, most < cache->n_pages ? most : cache->n_pages)), kCopyThreads, 0, s, *cache, plan,
+                         false, ctx->status_dev);
 }
 
 extern "C" int dc_kv8_free(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, const uint32_t* seqs, uint32_t n) {
@@ -503,8 +482,7 @@ extern "C" int dc_kv8_free(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache,
     if (n == 0) return DC_OK;
     DC_REQUIRE(ctx, seqs, "kv8_free: null operand");
     const dc_device_scope scope(ctx);
-    free_kernel<<<n, 128, 0, static_cast<cudaStream_t>(stream)>>>(*cache, seqs, ctx->status_dev);
-    return dc_check_launch(ctx, "kv8_free");
+    return dc_kv8_launch(ctx, "kv8_free", free_kernel, true, dim3(n), 128, 0, static_cast<cudaStream_t>(stream), *cache, seqs, ctx->status_dev);
 }
 
 extern "C" int dc_kv8_compact(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t* live) {
@@ -515,8 +493,7 @@ extern "C" int dc_kv8_compact(dc_ctx* ctx, void* stream, const dc_kv8_cache* cac
     Plan plan;
     if ((rc = pages_begin(ctx, "kv8_compact", cache, &plan)) != DC_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    compact_kernel<<<1, kPlanThreads, 0, s>>>(*cache, plan, live);
-    if ((rc = dc_check_launch(ctx, "kv8_compact")) != DC_OK) return rc;
+    if ((rc = dc_kv8_launch(ctx, "kv8_compact", compact_kernel, true, dim3(1), kPlanThreads, 0, s, *cache, plan, live)) != DC_OK) return rc;
     // at most half of the pages move
-    return launch_copies(ctx, s, "kv8_compact (copies)", copy_grid(ctx, cache, cache->n_pages / 2 + 1), *cache, plan, true);
+    return dc_kv8_launch(ctx, "kv8_compact (copies)", copy_kernel, true, dim3(copy_grid(ctx, cache, cache->n_pages / 2 + 1)), kCopyThreads, 0, s, *cache, plan, true, ctx->status_dev);
 }
