@@ -503,7 +503,8 @@ uint32_t longest(const dc_kv8_cache* c, uint32_t max_len) {
 // over 8,000 24.8 and 28.3; of 256 pairs over 600 keys 19.5 and 10.8, over 2,307 22.3 and 25.1; 16 sequences of 64 pairs over 1,000
 // keys 28 and 36; 64 of 24 pairs over 1,200 keys 150 and 67. Heads of 256, 4 kv heads: 64 pairs over 8,000 keys 29.3 and 27.9; 16
 // sequences of 64 pairs over 1,000 keys 29 and 48.
-bool on_tcgen05(const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
+bool on_tcgen05(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t max_q, uint32_t max_len) {
+    if (ctx->attn_engine != DC_ENGINE_TCGEN05) return false;
     const double pairs = static_cast<double>(max_q) * (nq / c->nkv);
     return pairs >= 64 && pairs * c->n_seqs * c->nkv * max_len * c->hd >= 536870912.0;
 }
@@ -526,7 +527,7 @@ int dc_kv8_attention_warm(dc_ctx* ctx) {
 extern "C" size_t dc_kv8_attention_scratch_bytes(dc_ctx* ctx, const dc_kv8_cache* cache, uint32_t nq, uint32_t max_q, uint32_t max_len) {
     if (!ctx || dc_kv8_check(cache, nullptr, 0) != DC_OK || nq == 0 || nq % cache->nkv || max_q == 0) return 0;
     const uint32_t len = longest(cache, max_len);
-    return (on_tcgen05(cache, nq, max_q, len) ? dc_kv8_attention_tc_cut(ctx, cache, nq, max_q, len) : cut_of(ctx, cache, nq, max_q, len)).part_bytes;
+    return (on_tcgen05(ctx, cache, nq, max_q, len) ? dc_kv8_attention_tc_cut(ctx, cache, nq, max_q, len) : cut_of(ctx, cache, nq, max_q, len)).part_bytes;
 }
 
 extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t layer, const void* q, const float* gate,
@@ -546,13 +547,12 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
                "kv8_attention: ldg = %u must cover the gate columns and be a multiple of 4, gate 16-byte aligned", ldg);
     DC_REQUIRE(ctx, reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0, "kv8_attention: q and y must be 16-byte aligned");
     if (rows == 0 || max_q == 0) return DC_OK;   // no rows: nothing to write
-    const uint32_t most = max_q < rows ? max_q : rows;
-    if (static_cast<uint64_t>(most) * (nq / cache->nkv) >= (1ull << 28))
-        return dc_fail(ctx, DC_UNSUPPORTED, "kv8_attention: %u rows of %u heads per kv head in one sequence (below 2^28 together)", most, nq / cache->nkv);
+    if (static_cast<uint64_t>(max_q) * (nq / cache->nkv) >= (1ull << 28))
+        return dc_fail(ctx, DC_UNSUPPORTED, "kv8_attention: max_q = %u rows of %u heads per kv head (below 2^28 together)", max_q, nq / cache->nkv);
     const dc_device_scope scope(ctx);
     const uint32_t len = longest(cache, max_len);
-    const bool tc = on_tcgen05(cache, nq, most, len);
-    const Kv8Cut t = tc ? dc_kv8_attention_tc_cut(ctx, cache, nq, most, len) : cut_of(ctx, cache, nq, most, len);
+    const bool tc = on_tcgen05(ctx, cache, nq, max_q, len);
+    const Kv8Cut t = tc ? dc_kv8_attention_tc_cut(ctx, cache, nq, max_q, len) : cut_of(ctx, cache, nq, max_q, len);   // as dc_kv8_attention_scratch_bytes says
     DC_REQUIRE(ctx, t.ctas < 0x7fffffffull, "kv8_attention: %llu CTAs: fewer rows or sequences a call", static_cast<unsigned long long>(t.ctas));
     Kv8Args a;
     a.c = *cache;
@@ -574,7 +574,7 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     a.qpos = qpos;
     a.y = static_cast<uint16_t*>(y);
     a.status = ctx->status_dev;
-    a.rows = rows, a.ldq = ldq, a.ldg = ldg, a.ldy = ldy, a.group = nq / cache->nkv, a.max_q = most, a.max_len = len;
+    a.rows = rows, a.ldq = ldq, a.ldg = ldg, a.ldy = ldy, a.group = nq / cache->nkv, a.max_q = max_q, a.max_len = len;
     a.tiles = t.tiles, a.chunk = t.chunk, a.chunks = t.chunks;
     a.page_shift = __builtin_ctz(cache->page_size), a.group_inverse = a.group > 1 ? static_cast<uint32_t>((1ull << 32) / a.group + 1) : 0u;
     a.scale = kKv8Log2e / sqrtf(static_cast<float>(cache->hd));

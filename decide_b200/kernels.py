@@ -105,6 +105,7 @@ class Kv8Cache:
         self.struct = _Kv8Struct(*(t.data_ptr() for t in (k, v, k_scale, v_scale, table, lens, refs)), *(k.stride(i) for i in range(4)), layers, n_pages, nkv,
                                  page_size, hd, *table.shape, 0)
         self.ref = ctypes.addressof(self.struct)
+        self.device = k.device.index   # None on the CPU (a description to check)
         err = ctypes.create_string_buffer(160)
         rc = _lib.load().dc_kv8_check(self.ref, err, len(err))
         if rc != 0:
@@ -423,31 +424,36 @@ class Kv8(_Family):
         # the handle of torch's current stream without a Stream object around it: 0.1 us instead of 1.3, a fifth of a short call
         return torch._C._cuda_getCurrentRawStream(self.dev.device) if stream is None else _stream(stream)
 
+    def _ref(self, cache: Kv8Cache) -> int:
+        if cache.device != self.dev.device:
+            raise KernelError(1, f"Kv8: the cache is on device {cache.device}, the context on {self.dev.device}")
+        return cache.ref
+
     def extend(self, stream, cache: Kv8Cache, add):
         """Lengthens sequence j by add[j] tokens: gives it the pages it lacks."""
-        self.dev.call("dc_kv8_extend", self._stream(stream), cache.ref, _ptr(add))
+        self.dev.call("dc_kv8_extend", self._stream(stream), self._ref(cache), _ptr(add))
 
     def fork(self, stream, cache: Kv8Cache, src, dst, n: int, deep: bool = False):
         """Sequence dst[i] becomes a copy of src[i]: it shares the full pages (deep: gets copies of all)."""
-        self.dev.call("dc_kv8_fork", self._stream(stream), cache.ref, _ptr(src), _ptr(dst), n, int(deep))
+        self.dev.call("dc_kv8_fork", self._stream(stream), self._ref(cache), _ptr(src), _ptr(dst), n, int(deep))
 
     def free(self, stream, cache: Kv8Cache, seqs, n: int):
         """Frees sequences seqs[0 .. n)."""
-        self.dev.call("dc_kv8_free", self._stream(stream), cache.ref, _ptr(seqs), n)
+        self.dev.call("dc_kv8_free", self._stream(stream), self._ref(cache), _ptr(seqs), n)
 
     def compact(self, stream, cache: Kv8Cache, live=None):
         """Moves the pages in use to the lowest ids; live[0] (int32, may be None) receives how many there are."""
-        self.dev.call("dc_kv8_compact", self._stream(stream), cache.ref, _ptr(live))
+        self.dev.call("dc_kv8_compact", self._stream(stream), self._ref(cache), _ptr(live))
 
     def append(self, stream, cache: Kv8Cache, layer: int, k, v, ldk: int, ldv: int, row_start, rows: int, max_rows: int):
         """Writes rows row_start[j] .. row_start[j+1] of k and v as the last tokens of sequence j."""
-        self.dev.call("dc_kv8_append", self._stream(stream), cache.ref, layer, _ptr(k), _ptr(v), ldk, ldv, _ptr(row_start), rows, max_rows)
+        self.dev.call("dc_kv8_append", self._stream(stream), self._ref(cache), layer, _ptr(k), _ptr(v), ldk, ldv, _ptr(row_start), rows, max_rows)
 
     def attention(self, stream, cache: Kv8Cache, layer: int, q, gate, q_start, qpos, y, rows: int, ldq: int, ldg: int, ldy: int, nq: int, max_q: int,
                   max_len: int = 0):
         """Causal GQA attention of rows q_start[j] .. q_start[j+1] over sequence j, with the optional sigmoid gate; qpos None: the rows
         are the sequence's last tokens."""
-        self.dev.call("dc_kv8_attention", self._stream(stream), cache.ref, layer, _ptr(q), _ptr(gate), _ptr(q_start), _ptr(qpos), _ptr(y), rows, ldq, ldg,
+        self.dev.call("dc_kv8_attention", self._stream(stream), self._ref(cache), layer, _ptr(q), _ptr(gate), _ptr(q_start), _ptr(qpos), _ptr(y), rows, ldq, ldg,
                       ldy, nq, max_q, max_len)
 
     def pages_scratch_bytes(self, cache: Kv8Cache) -> int:

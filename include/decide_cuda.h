@@ -97,7 +97,7 @@ int dc_set_delta_split(dc_ctx* ctx, uint32_t split);
  *    also splits the value columns over CTAs. Same results to ~1e-6.
  *  DC_FAMILY_ATTN: tcgen05 serves packed batches (seq_start given) and chunks of one sequence whose cache
  *    length is given (dc_attention); other calls without seq_start run on mma.sync. Same contract;
- *    results differ by fp32 rounding order only.
+ *    results differ by fp32 rounding order only. dc_kv8_attention with many rows likewise.
  *  DC_FAMILY_GEMM has one engine (tcgen05). */
 int dc_set_engine(dc_ctx* ctx, uint32_t family, uint32_t engine);
 /* Synchronises `stream`, then reports DC_TIMEOUT if a kernel's bounded wait ran out since the
@@ -437,8 +437,11 @@ int dc_kv8_append(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t
  * are); a page id outside the pool makes the rows that attend it NaN. scale hd^-1/2, fp32 scores and softmax; the weights of the
  * V product are rounded to fp16 (they are at most 2^8 of the row's largest term). `gate` (fp32, row stride ldg, NULL = none)
  * multiplies the output by sigmoid(gate). Writes rows below q_start[n_seqs] of y (the 16-bit type, row stride ldy), no others.
- * nq / nkv <= 16; q, y, gate 16-byte aligned, ldq, ldy multiples of 8, ldg of 4, each >= nq * hd. max_len: the longest
- * sequence, or more (it sizes the split of the keys; 0 = max_pages * page_size); a longer one is a violation. Scratch: dc_kv8_attention_scratch_bytes. */
+ * nq / nkv <= 16, max_q * nq / nkv < 2^28; q, y, gate 16-byte aligned, ldq, ldy multiples of 8, ldg of 4, each >= nq * hd. max_len: the longest
+ * sequence, or more (it sizes the split of the keys; 0 = max_pages * page_size); a longer one is a violation. Scratch:
+ * dc_kv8_attention_scratch_bytes of the same nq, max_q and max_len. From 64 (row, head) pairs of a kv head in a sequence and enough
+ * keys on it runs on tcgen05 unless dc_set_engine says DC_ENGINE_MMA_SYNC for DC_FAMILY_ATTN (the two agree to fp32 rounding order and
+ * the rounding of the weights). The result does not depend on timing: the same call gives the same bits. */
 int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t layer, const void* q, const float* gate,
                      const uint32_t* q_start, const uint32_t* qpos, void* y, uint32_t rows, uint32_t ldq, uint32_t ldg, uint32_t ldy,
                      uint32_t nq, uint32_t max_q, uint32_t max_len);

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from decide_b200.kernels import KernelError, Kv8Cache
+from decide_b200.kernels import Engine, Family, KernelError, Kv8Cache
 from oracle import kv8
 
 pytestmark = pytest.mark.gpu
@@ -272,6 +272,15 @@ def test_append_non_finite_poisons_its_page_and_head_alone(k, act):
     k.dev.check_status()
 
 
+def test_a_cache_elsewhere_is_refused(k):
+    """The context's device and the cache's have to be the same."""
+    p = Pair(k)
+    cpu = Kv8Cache.empty(1, 4, 2, 128, 3, 4, 16, device="cpu")
+    for call in (lambda: p.ops.extend(None, cpu, p.ints([0, 0, 0])), lambda: p.ops.compact(None, cpu), lambda: p.ops.free(None, cpu, p.ints([0]), 1)):
+        with pytest.raises(KernelError, match="device"):
+            call()
+
+
 def test_append_refusals(k):
     p = Pair(k)
     x = torch.zeros(4, 264, dtype=k.dev.act_torch, device="cuda")
@@ -401,6 +410,25 @@ def test_attention_repeats_bit_for_bit(k, hd):
     k.dev.check_status()
 
 
+def test_attention_engines_agree(k):
+    """dc_set_engine keeps a call off tcgen05; what scratch_bytes says is what the call takes, on either."""
+    p = _filled(k, [1500, 700], 2, 128, 32, room=ROOM)
+    counts, nq = [60, 33], 8
+    try:
+        for engine in (Engine.Tcgen05, Engine.MmaSync):
+            k.dev.set_engine(Family.Attn, engine)
+            k.dev.reserve_workspace(p.ops.attention_scratch_bytes(p.gpu, nq, 60, 0))
+            k.dev.set_workspace_frozen(True)
+            before = k.dev.launches
+            p.attend(counts, nq, max_len=0)
+            assert k.dev.launches - before == (2 if engine == Engine.Tcgen05 else 1)      # cut in chunks there, whole or joined in place here
+            k.dev.set_workspace_frozen(False)
+        k.dev.check_status()
+    finally:
+        k.dev.set_workspace_frozen(False)
+        k.dev.set_engine(Family.Attn, Engine.Tcgen05)
+
+
 def test_attention_one_key_is_its_value(k):
     """A row that sees one key gets that key's V: codes times scale, exactly (they fit fp16)."""
     p = _filled(k, [1], 2, 128, 16)
@@ -489,7 +517,7 @@ def test_attention_refusals(k):
     p.ops.attention(None, p.gpu, **{**good, "rows": 0})
     p.ops.attention(None, p.gpu, **{**good, "max_q": 0})
     for bad in ({"layer": 1}, {"q": None}, {"q_start": None}, {"y": None}, {"nq": 7}, {"nq": 0}, {"nq": 34}, {"ldq": 1016}, {"ldq": 1028}, {"ldy": 1020}, {"ldg": 1022},
-                {"ldg": 512}, {"q": (q, 8)}, {"y": (y, 2)}, {"gate": (g, 4)}):
+                {"ldg": 512}, {"q": (q, 8)}, {"y": (y, 2)}, {"gate": (g, 4)}, {"max_q": 1 << 27}):
         with pytest.raises(KernelError):
             p.ops.attention(None, p.gpu, **{**good, **bad})
     k.dev.check_status()
