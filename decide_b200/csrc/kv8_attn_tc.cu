@@ -18,6 +18,9 @@
 // both with one tile of 128 pairs (O has 256 columns) and stages of 64 keys; warps 5..7 then help the fillers, who have twice the codes for
 // each product (with three of them a half took 3,500 cycles).
 // Where there are fewer tiles than SMs the keys are cut into chunks, whose results a second kernel joins in chunk order.
+// Measured on the device, 32 query heads of 128 over 8 kv heads: 2,048 rows over 8,191 keys 300 us (800 TFLOP/s; tensor pipe 35 % busy, of 43 %
+// that 256 CTAs on 148 SMs allow), 178 rows over 2,491 keys 28 us; kv8_attn.cu takes 1,062 and 51. A round of both tiles' 64 keys takes
+// 2,050 cycles, its MMAs alone 1,250 (128x64x16 with both operands in shared memory 48 each, 128x128x16 with A in tensor memory 64).
 // Every wait is bounded; when one gives up the CTA raises the status word, waits for its products in flight and returns.
 #include "kv8_attn.cuh"
 #include "ptx.cuh"
