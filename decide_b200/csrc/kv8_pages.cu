@@ -8,8 +8,9 @@
 //
 // What bounds them: the deciding CTA is a chain of a few block-wide steps (latency; refs are read 16 bytes a thread), the copying
 // kernel is bound by memory (a page-head block of page_size * hd codes, contiguous in the default layout, per warp step).
-// Measured on the device: copies of four states of 2,307 tokens in nine layers 64 us (350 MB at 6.2 TB/s in the copying kernel); eight forks
-// that share, grow, half of them freed, the cache closed up: 27.6 us in six kernels.
+// Measured on the device: copies of four states of 2,307 tokens in nine layers 62 us (350 MB, 5.7 TB/s with
+// the deciding kernel); eight forks that share, grow, half of them freed, the cache closed up: 24 us in six kernels (27.6 with the forks'
+// sequences and lengths loaded again by each step, and rows split by divisions in the copying kernel).
 #include "kv8.cuh"
 
 namespace {
@@ -84,23 +85,20 @@ __device__ uint32_t find_free(const uint32_t* refs, uint32_t n_pages, uint32_t n
 // A sequence's pages, from its length as it is now; flags a length that its row of the table cannot hold.
 __device__ __forceinline__ bool length_fits(const dc_kv8_cache& c, uint32_t len) { return len <= c.max_pages * c.page_size; }
 
-// refs of the pages of sequences ids[0 .. n): `by` = -1 gives them up, + 1 takes them back. Warps take the sequences in turn. *bad is set
-// where a page id is outside the pool (it is passed over) or a page that nobody held is given up.
-__device__ __forceinline__ void release(const dc_kv8_cache& c, const uint32_t* ids, uint32_t n, int by, int* bad) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (uint32_t i = warp; i < n; i += kPlanThreads / 32) {
-        const uint32_t j = ids[i], pages = kv8_pages(c.lens[j], c.page_size);
-        for (uint32_t col = lane; col < pages; col += 32) {
-            const uint32_t page = c.table[static_cast<size_t>(j) * c.max_pages + col];
-            if (page >= c.n_pages) *bad = DC_STATUS_KV8_PAGE;
-            else if (atomicAdd(&c.refs[page], static_cast<uint32_t>(by)) == 0u && by < 0) *bad = DC_STATUS_KV8_REFS;
-        }
+// refs of the pages of sequence j of `len` tokens, by one warp: `by` = -1 gives them up, + 1 takes them back, 0 only looks at the table. *bad is
+// set where a page id is outside the pool (it is passed over) or a page that nobody held is given up.
+__device__ __forceinline__ void hold(const dc_kv8_cache& c, uint32_t j, uint32_t len, int by, int* bad) {
+    const uint32_t pages = kv8_pages(len, c.page_size);
+    for (uint32_t col = threadIdx.x & 31; col < pages; col += 32) {
+        const uint32_t page = c.table[static_cast<size_t>(j) * c.max_pages + col];
+        if (page >= c.n_pages) *bad = DC_STATUS_KV8_PAGE;
+        else if (by != 0 && atomicAdd(&c.refs[page], static_cast<uint32_t>(by)) == 0u && by < 0) *bad = DC_STATUS_KV8_REFS;
     }
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
 extend_kernel(dc_kv8_cache c, const uint32_t* __restrict__ add, Plan plan, int* __restrict__ status) {
-    __shared__ uint32_t sums[64];
+    __shared__ uint32_t sums[64], few[kPlanThreads];
     __shared__ int bad;
     uint32_t turn = 0;
     kv8_begin();
@@ -131,7 +129,8 @@ extend_kernel(dc_kv8_cache c, const uint32_t* __restrict__ add, Plan plan, int* 
         need = min(need + total, c.n_pages + 1);   // more than the pool is too many, however many
     }
     __syncthreads();
-    if (bad || need > c.n_pages || find_free(c.refs, c.n_pages, need, plan.slots, sums, turn) < need) {
+    uint32_t* slots = need <= kPlanThreads ? few : plan.slots;
+    if (bad || need > c.n_pages || find_free(c.refs, c.n_pages, need, slots, sums, turn) < need) {
         if (threadIdx.x == 0) kv8_flag(status, bad ? bad : DC_STATUS_KV8_POOL);
         return;
     }
@@ -145,7 +144,7 @@ extend_kernel(dc_kv8_cache c, const uint32_t* __restrict__ add, Plan plan, int* 
         }
         const uint32_t j = base + threadIdx.x;
         for (uint32_t i = 0; i < mine; ++i) {
-            const uint32_t page = plan.slots[place + i];
+            const uint32_t page = slots[place + i];
             c.table[static_cast<size_t>(j) * c.max_pages + held + i] = page;
             c.refs[page] = 1u;
         }
@@ -161,9 +160,11 @@ __device__ __forceinline__ uint32_t copied_pages(const dc_kv8_cache& c, uint32_t
 __global__ void __launch_bounds__(kPlanThreads)
 fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __restrict__ dst, uint32_t n, bool deep, Plan plan, int* __restrict__ status) {
     extern __shared__ uint32_t taken[];   // one bit a sequence: it is a destination
-    __shared__ uint32_t sums[64];
+    __shared__ uint32_t sums[64], few[kPlanThreads], places[kPlanThreads];
+    __shared__ uint4 named[kPlanThreads];   // of up to 1024 forks: source, destination, their lengths (each step would load them again otherwise)
     __shared__ int bad;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool one_round = n <= kPlanThreads;
     uint32_t turn = 0;
     kv8_begin();
     for (uint32_t i = threadIdx.x; i < (c.n_seqs + 31) / 32; i += kPlanThreads) taken[i] = 0u;
@@ -186,14 +187,16 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
                 if (atomicOr(&taken[d >> 5], 1u << (d & 31)) >> (d & 31) & 1u) bad = DC_STATUS_KV8_SEQUENCE;
                 if (!length_fits(c, d_len) || !length_fits(c, s_len)) bad = DC_STATUS_KV8_LENGTH;
                 else copied = min(copied_pages(c, s_len, deep), c.n_pages + 1);
+                named[threadIdx.x] = make_uint4(s, d, s_len, d_len);
             }
         }
         place = block_scan(copied, sums, turn, &total);
+        places[threadIdx.x] = place;   // read as they are where there is one round
         need = min(need + total, c.n_pages + 1);
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n && !bad; i += kPlanThreads) {
-        const uint32_t s = src[i];
+        const uint32_t s = one_round ? named[i].x : src[i];
         if (taken[s >> 5] >> (s & 31) & 1u) bad = DC_STATUS_KV8_SEQUENCE;
     }
     __syncthreads();
@@ -201,46 +204,54 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
         if (threadIdx.x == 0) kv8_flag(status, bad);
         return;
     }
+    auto fork_at = [&](uint32_t i) {   // as named[i], past the first 1024 too
+        if (one_round) return named[i];
+        const uint32_t s = src[i], d = dst[i];
+        return make_uint4(s, d, c.lens[s], c.lens[d]);
+    };
     // the destinations give up what they hold; what the sources hold has to name pages
-    release(c, dst, n, -1, &bad);
-    for (uint32_t i = warp; i < n; i += kPlanThreads / 32) {
-        const uint32_t j = src[i], pages = kv8_pages(c.lens[j], c.page_size);
-        for (uint32_t col = lane; col < pages; col += 32)
-            if (c.table[static_cast<size_t>(j) * c.max_pages + col] >= c.n_pages) bad = DC_STATUS_KV8_PAGE;
+    for (uint32_t i = warp; i < 2 * n; i += kPlanThreads / 32) {
+        const uint4 f = fork_at(i >> 1);
+        if (i & 1u) hold(c, f.y, f.w, -1, &bad);
+        else hold(c, f.x, f.z, 0, &bad);
     }
     __syncthreads();
-    const bool enough = !bad && need <= c.n_pages && find_free(c.refs, c.n_pages, need, plan.slots, sums, turn) == need;
+    uint32_t* slots = need <= kPlanThreads ? few : plan.slots;
+    const bool enough = !bad && need <= c.n_pages && find_free(c.refs, c.n_pages, need, slots, sums, turn) == need;
     __syncthreads();
     if (!enough) {   // as it was
         const int what = bad ? bad : DC_STATUS_KV8_POOL;
         __syncthreads();
-        release(c, dst, n, 1, &bad);
+        for (uint32_t i = warp; i < n; i += kPlanThreads / 32) {
+            const uint4 f = fork_at(i);
+            hold(c, f.y, f.w, 1, &bad);
+        }
         if (threadIdx.x == 0) kv8_flag(status, what);
         return;
     }
     uint32_t given = 0;
     for (uint32_t base = 0; base < n; base += kPlanThreads) {
-        if (n > kPlanThreads) {   // otherwise the one round above still stands
+        if (!one_round) {
             const uint32_t i = base + threadIdx.x;
             uint32_t total;
-            place = given + block_scan(i < n ? copied_pages(c, c.lens[src[i]], deep) : 0u, sums, turn, &total);
+            place = given + block_scan(i < n ? copied_pages(c, fork_at(i).z, deep) : 0u, sums, turn, &total);
             given += total;
+            __syncthreads();
+            places[threadIdx.x] = place;
+            __syncthreads();
         }
         // warps over the round's forks, lanes over the pages; a fork's place comes from the warp that scanned it
-        __shared__ uint32_t places[kPlanThreads];
-        __syncthreads();
-        places[threadIdx.x] = place;
-        __syncthreads();
         for (uint32_t k = warp; k < kPlanThreads && base + k < n; k += kPlanThreads / 32) {
-            const uint32_t at = base + k, s = src[at], len = c.lens[s], pages = kv8_pages(len, c.page_size), copied = copied_pages(c, len, deep), shared = pages - copied;
-            const uint32_t* from = c.table + static_cast<size_t>(s) * c.max_pages;
-            uint32_t* to = c.table + static_cast<size_t>(dst[at]) * c.max_pages;
+            const uint4 f = fork_at(base + k);
+            const uint32_t pages = kv8_pages(f.z, c.page_size), copied = copied_pages(c, f.z, deep), shared = pages - copied;
+            const uint32_t* from = c.table + static_cast<size_t>(f.x) * c.max_pages;
+            uint32_t* to = c.table + static_cast<size_t>(f.y) * c.max_pages;
             for (uint32_t col = lane; col < pages; col += 32) {
                 uint32_t page = from[col];
                 if (col < shared) {
                     atomicAdd(&c.refs[page], 1u);
                 } else {
-                    const uint32_t slot = places[k] + col - shared, fresh = plan.slots[slot];
+                    const uint32_t slot = places[k] + col - shared, fresh = slots[slot];
                     plan.moves[slot] = make_uint2(page, fresh);
                     c.refs[fresh] = 1u;
                     page = fresh;
@@ -249,8 +260,11 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
             }
         }
     }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) c.lens[dst[i]] = c.lens[src[i]];
+    __syncthreads();   // `lens` are read above where there are several rounds
+    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
+        if (one_round) c.lens[named[i].y] = named[i].z;
+        else c.lens[dst[i]] = c.lens[src[i]];
+    }
     if (threadIdx.x == 0) plan.head[0] = need;
 }
 
@@ -330,6 +344,17 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(dc_kv8_cache c, P
     }
 }
 
+// a = *quotient * b + remainder. Divided in 32 bits where it fits, which the units of a call nearly always do.
+__device__ __forceinline__ uint32_t split(uint64_t a, uint32_t b, uint64_t* quotient) {
+    if (a >> 32) {
+        *quotient = a / b;
+        return static_cast<uint32_t>(a % b);
+    }
+    const uint32_t q = static_cast<uint32_t>(a) / b;
+    *quotient = q;
+    return static_cast<uint32_t>(a) - q * b;
+}
+
 // Copies the listed pages in every layer; with `rename` also rewrites the table. A warp takes one (move, layer, K or V, head) at a time:
 // page_size * hd codes and a scale. No page is both read and written (the lists are made so).
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(dc_kv8_cache c, Plan plan, bool rename, int* __restrict__ status) {
@@ -337,14 +362,14 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(dc_kv8_cache c, Plan
     kv8_begin();
     const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kCopyThreads / 32);
     const uint64_t units = static_cast<uint64_t>(plan.head[0]) * c.layers * 2 * c.nkv;
-    const uint32_t per_row = c.hd / 16, vectors = c.page_size * per_row;
+    const uint32_t row_bits = c.hd == 256 ? 4 : 3, in_row = (1u << row_bits) - 1, vectors = c.page_size << row_bits;   // a row of codes is 8 or 16 vectors
     const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (kCopyThreads / 32) + (threadIdx.x >> 5);
     for (uint64_t u = first; u < units; u += warps) {
-        const uint32_t head = static_cast<uint32_t>(u % c.nkv);
-        const uint64_t rest = u / c.nkv;
+        uint64_t rest, move;
+        const uint32_t head = split(u, c.nkv, &rest);
         const bool is_v = rest & 1u;
-        const uint32_t layer = static_cast<uint32_t>((rest >> 1) % c.layers);
-        const uint2 mv = plan.moves[(rest >> 1) / c.layers];
+        const uint32_t layer = split(rest >> 1, c.layers, &move);
+        const uint2 mv = plan.moves[move];
         uint8_t* base = static_cast<uint8_t*>(is_v ? c.v : c.k) + layer * c.layer_stride + head * c.head_stride;
         const uint8_t* from = base + mv.x * c.page_stride;
         uint8_t* to = base + mv.y * c.page_stride;
@@ -353,12 +378,12 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(dc_kv8_cache c, Plan
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t w = e + 32 * i;
-                if (w < vectors) x[i] = *reinterpret_cast<const uint4*>(from + (w / per_row) * c.token_stride + 16 * (w % per_row));
+                if (w < vectors) x[i] = *reinterpret_cast<const uint4*>(from + (w >> row_bits) * c.token_stride + 16 * (w & in_row));
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t w = e + 32 * i;
-                if (w < vectors) *reinterpret_cast<uint4*>(to + (w / per_row) * c.token_stride + 16 * (w % per_row)) = x[i];
+                if (w < vectors) *reinterpret_cast<uint4*>(to + (w >> row_bits) * c.token_stride + 16 * (w & in_row)) = x[i];
             }
         }
         if (lane == 0) {
