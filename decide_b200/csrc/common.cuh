@@ -23,6 +23,9 @@ typedef CUresult (*dc_encode_tiled_fn)(CUtensorMap*, CUtensorMapDataType, cuuint
 // (base pointer, rows, cols, row stride in elements, box rows)
 typedef std::tuple<const void*, uint32_t, uint32_t, uint32_t, uint32_t> dc_tmap_key;
 
+#define DC_KV8_DONE_COUNTERS 65536u
+#define DC_WORKSPACES_SET_ASIDE 16u
+
 struct dc_ctx {
     int device = 0;
     int sm_count = 0;
@@ -46,6 +49,9 @@ struct dc_ctx {
     void* workspace = nullptr;       // scratch for the chunked delta rule and other multi-pass ops
     size_t workspace_bytes = 0;
     bool workspace_frozen = false;   // an op that needs more scratch than is reserved fails instead of allocating
+    bool workspace_captured = false; // a captured graph holds the workspace: growing it sets it aside until dc_close
+    void* set_aside[DC_WORKSPACES_SET_ASIDE] = {};
+    uint32_t set_aside_count = 0;
     uint64_t allocs = 0;             // device/pinned allocations this context made (dc_open, workspace growth)
     uint64_t tmap_encodes = 0;       // tensor maps encoded (cache misses)
     void* tp_comm = nullptr;         // NCCL communicator of the tensor-parallel group (dc_tp_init), or null
@@ -53,7 +59,6 @@ struct dc_ctx {
     bool tp_exchange16 = false;      // partial sums cross the links in the 16-bit type (half the bytes) instead of fp32
 };
 
-#define DC_KV8_DONE_COUNTERS 65536u
 
 int dc_fail(dc_ctx* ctx, int code, const char* fmt, ...);
 int dc_check_launch(dc_ctx* ctx, const char* what);

@@ -33,7 +33,15 @@ int dc_get_workspace(dc_ctx* ctx, size_t bytes, const char* who, void** out) {
     if (ctx->workspace_frozen)
         return dc_fail(ctx, DC_INVALID_ARG, "%s: needs %zu bytes of scratch but the workspace is frozen at %zu (reserve more with dc_reserve_workspace before freezing)",
                        who, bytes, ctx->workspace_bytes);
-    if (ctx->workspace) cudaFree(ctx->workspace);
+    if (ctx->workspace_captured) {
+        if (ctx->set_aside_count == DC_WORKSPACES_SET_ASIDE)
+            return dc_fail(ctx, DC_INVALID_ARG, "%s: needs %zu bytes of scratch, and the workspace has grown %u times under captured graphs already (reserve more with dc_reserve_workspace)",
+                           who, bytes, DC_WORKSPACES_SET_ASIDE);
+        ctx->set_aside[ctx->set_aside_count++] = ctx->workspace;
+        ctx->workspace_captured = false;
+    } else if (ctx->workspace) {
+        cudaFree(ctx->workspace);
+    }
     ctx->workspace = nullptr;
     ctx->workspace_bytes = 0;
     void* p = nullptr;
@@ -46,6 +54,17 @@ int dc_get_workspace(dc_ctx* ctx, size_t bytes, const char* who, void** out) {
     ctx->workspace_bytes = bytes ? bytes : 256;
     *out = p;
     return DC_OK;
+}
+
+int dc_kv8_workspace(dc_ctx* ctx, cudaStream_t stream, size_t bytes, const char* who, void** out) {
+    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &state) != cudaSuccess) cudaGetLastError();   // the default stream while another one captures
+    const bool captured = state == cudaStreamCaptureStatusActive;
+    if (captured && !ctx->workspace_frozen && (bytes > ctx->workspace_bytes || !ctx->workspace))
+        return dc_fail(ctx, DC_INVALID_ARG, "%s: needs %zu bytes of scratch, which cannot be allocated during a capture (reserve them with dc_reserve_workspace)", who, bytes);
+    const int rc = dc_get_workspace(ctx, bytes, who, out);
+    if (rc == DC_OK && captured) ctx->workspace_captured = true;
+    return rc;
 }
 
 // Messages of the violations that only the dc_kv8_* kernels can see; null for other codes.
@@ -155,7 +174,8 @@ dc_ctx* dc_open(int device, char* err, size_t err_len) {
     }
     ctx->allocs += 2;
     if ((e = cudaMalloc(&ctx->kv8_done, DC_KV8_DONE_COUNTERS * sizeof(uint32_t))) != cudaSuccess ||
-        (e = cudaMemset(ctx->kv8_done, 0, DC_KV8_DONE_COUNTERS * sizeof(uint32_t))) != cudaSuccess) {
+        (e = cudaMemset(ctx->kv8_done, 0, DC_KV8_DONE_COUNTERS * sizeof(uint32_t))) != cudaSuccess ||
+        (e = cudaStreamSynchronize(nullptr)) != cudaSuccess) {   // the caller's streams do not wait for these memsets by themselves
         say("dc_open: cannot allocate the attention counters", cudaGetErrorString(e));
         dc_close(ctx);
         return nullptr;
@@ -171,6 +191,7 @@ void dc_close(dc_ctx* ctx) {
     if (ctx->status_dev) cudaFree(ctx->status_dev);
     if (ctx->status_host) cudaFreeHost(ctx->status_host);
     if (ctx->workspace) cudaFree(ctx->workspace);
+    for (uint32_t i = 0; i < ctx->set_aside_count; ++i) cudaFree(ctx->set_aside[i]);
     if (ctx->kv8_done) cudaFree(ctx->kv8_done);
     if (ctx->gemm_part_ws) cudaFree(ctx->gemm_part_ws);
     if (ctx->gemm_part_cnt) cudaFree(ctx->gemm_part_cnt);

@@ -68,6 +68,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+// A weight as the total counts it: rounded, as the V product takes it, so that what rounding does to a row that one key dominates cancels;
+// but exact where fp16 runs out of bits (below 2^-14 of the largest term), since a key whose page has a small V scale may weigh
+// much in the total and little in the product.
+__device__ __forceinline__ float kv8_total(float exact, float rounded) { return exact >= 6.103515625e-05f ? rounded : exact; }
+
 // One CTA: 8 NT (row, head) pairs of a sequence's kv head over one chunk of its keys.
 template <typename Act, int HD, int NT>
 __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlocks) kv8_attn_kernel(const Kv8Args a) {
@@ -517,9 +522,9 @@ bool on_tcgen05(const dc_ctx* ctx, const dc_kv8_cache* c, uint32_t nq, uint32_t 
 int dc_kv8_attention_warm(dc_ctx* ctx) {
     static bool set[16] = {};
     if (set[ctx->device & 15]) return DC_OK;
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t hd = i & 1 ? 256 : 128, nt = 1 + (i >> 1 & 3);
-        const Variant v = i & 8 ? pick<dc::ActF16>(hd, nt) : pick<dc::ActBF16>(hd, nt);
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t hd = i & 1 ? 256 : 128, nt = 1 + (i >> 1 & 1);
+        const Variant v = i & 4 ? pick<dc::ActF16>(hd, nt) : pick<dc::ActBF16>(hd, nt);
         const cudaError_t e = cudaFuncSetAttribute(v.f, cudaFuncAttributeMaxDynamicSharedMemorySize, v.bytes);
         if (e != cudaSuccess) return dc_fail(ctx, DC_CUDA_ERROR, "kv8_attention: cannot opt in to %d bytes of shared memory: %s", v.bytes, cudaGetErrorString(e));
     }
@@ -567,7 +572,7 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     a.done = ctx->kv8_done;
     if (t.chunks > 1) {
         void* ws = nullptr;
-        if ((rc = dc_get_workspace(ctx, t.part_bytes, "kv8_attention", &ws)) != DC_OK) return rc;
+        if ((rc = dc_kv8_workspace(ctx, static_cast<cudaStream_t>(stream), t.part_bytes, "kv8_attention", &ws)) != DC_OK) return rc;
         a.part = static_cast<float*>(ws);
     }
     if ((rc = dc_kv8_attention_warm(ctx)) != DC_OK) return rc;

@@ -72,11 +72,6 @@ struct Kv8Args {
 // pair / group: pairs are below 2^28 and groups at most 16, so the product with floor(2^32 / group) + 1 is exact.
 __device__ __forceinline__ uint32_t kv8_row_of(const Kv8Args& a, uint32_t pair) { return a.group == 1 ? pair : __umulhi(pair, a.group_inverse); }
 
-// A weight as the total counts it: rounded, as the V product takes it, so that what rounding does to a row that one key dominates cancels;
-// but exact where fp16 runs out of bits (below 2^-14 of the largest term), since a key whose page has a small V scale may weigh
-// much in the total and little in the product.
-__device__ __forceinline__ float kv8_total(float exact, float rounded) { return exact >= 6.103515625e-05f ? rounded : exact; }
-
 // The largest magnitude of a query row, as 16 bits; WORDS 8-byte pieces a lane holds of it, `lanes` (16 or 32) lanes hold the row.
 template <int WORDS>
 __device__ __forceinline__ uint32_t kv8_query_top(const uint2* x, int lanes = 32) {

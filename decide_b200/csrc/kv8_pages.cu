@@ -97,7 +97,7 @@ __device__ __forceinline__ void hold(const dc_kv8_cache& c, uint32_t j, uint32_t
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-extend_kernel(dc_kv8_cache c, const uint32_t* __restrict__ add, Plan plan, int* __restrict__ status) {
+extend_kernel(dc_kv8_cache c, const uint32_t* add, Plan plan, int* status) {
     __shared__ uint32_t sums[64], few[kPlanThreads];
     __shared__ int bad;
     uint32_t turn = 0;
@@ -158,7 +158,7 @@ __device__ __forceinline__ uint32_t copied_pages(const dc_kv8_cache& c, uint32_t
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __restrict__ dst, uint32_t n, bool deep, Plan plan, int* __restrict__ status) {
+fork_kernel(dc_kv8_cache c, const uint32_t* src, const uint32_t* dst, uint32_t n, bool deep, Plan plan, int* status) {
     extern __shared__ uint32_t taken[];   // one bit a sequence: it is a destination
     __shared__ uint32_t sums[64], few[kPlanThreads], places[kPlanThreads];
     __shared__ uint4 named[kPlanThreads];   // of up to 1024 forks: source, destination, their lengths (each step would load them again otherwise)
@@ -268,7 +268,7 @@ fork_kernel(dc_kv8_cache c, const uint32_t* __restrict__ src, const uint32_t* __
     if (threadIdx.x == 0) plan.head[0] = need;
 }
 
-__global__ void __launch_bounds__(128) free_kernel(dc_kv8_cache c, const uint32_t* __restrict__ seqs, int* __restrict__ status) {
+__global__ void __launch_bounds__(128) free_kernel(dc_kv8_cache c, const uint32_t* seqs, int* status) {
     kv8_begin();
     const uint32_t j = seqs[blockIdx.x];
     __shared__ uint32_t claimed;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(128) free_kernel(dc_kv8_cache c, const uint32_
     }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) compact_kernel(dc_kv8_cache c, Plan plan, uint32_t* __restrict__ live_out) {
+__global__ void __launch_bounds__(kPlanThreads) compact_kernel(dc_kv8_cache c, Plan plan, uint32_t* live_out) {
     __shared__ uint32_t sums[64];
     uint32_t turn = 0, live = 0, mask = 0;   // of four pages, those in use
     kv8_begin();
@@ -357,7 +357,7 @@ __device__ __forceinline__ uint32_t split(uint64_t a, uint32_t b, uint64_t* quot
 
 // Copies the listed pages in every layer; with `rename` also rewrites the table. A warp takes one (move, layer, K or V, head) at a time:
 // page_size * hd codes and a scale. No page is both read and written (the lists are made so).
-__global__ void __launch_bounds__(kCopyThreads) copy_kernel(dc_kv8_cache c, Plan plan, bool rename, int* __restrict__ status) {
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(dc_kv8_cache c, Plan plan, bool rename, int* status) {
     const uint32_t lane = threadIdx.x & 31;
     kv8_begin();
     const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kCopyThreads / 32);
@@ -414,9 +414,9 @@ uint32_t copy_grid(const dc_ctx* ctx, const dc_kv8_cache* c, uint64_t moves) {
     return static_cast<uint32_t>(ctas < 1 ? 1 : ctas < most ? ctas : most);
 }
 
-int pages_begin(dc_ctx* ctx, const char* who, const dc_kv8_cache* cache, Plan* plan) {
+int pages_begin(dc_ctx* ctx, void* stream, const char* who, const dc_kv8_cache* cache, Plan* plan) {
     void* ws = nullptr;
-    const int rc = dc_get_workspace(ctx, plan_bytes(cache->n_pages), who, &ws);
+    const int rc = dc_kv8_workspace(ctx, static_cast<cudaStream_t>(stream), plan_bytes(cache->n_pages), who, &ws);
     if (rc == DC_OK) *plan = plan_at(ws, cache->n_pages);
     return rc;
 }
@@ -479,7 +479,7 @@ extern "C" int dc_kv8_extend(dc_ctx* ctx, void* stream, const dc_kv8_cache* cach
     DC_REQUIRE(ctx, add, "kv8_extend: null operand");
     const dc_device_scope scope(ctx);
     Plan plan;
-    if ((rc = pages_begin(ctx, "kv8_extend", cache, &plan)) != DC_OK) return rc;
+    if ((rc = pages_begin(ctx, stream, "kv8_extend", cache, &plan)) != DC_OK) return rc;
     return dc_kv8_launch(ctx, "kv8_extend", extend_kernel, true, dim3(1), kPlanThreads, 0, static_cast<cudaStream_t>(stream), *cache, add, plan, ctx->status_dev);
 }
 
@@ -493,7 +493,7 @@ extern "C" int dc_kv8_fork(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache,
     DC_REQUIRE(ctx, n <= cache->n_seqs, "kv8_fork: %u forks of %u sequences", n, cache->n_seqs);
     const dc_device_scope scope(ctx);
     Plan plan;
-    if ((rc = pages_begin(ctx, "kv8_fork", cache, &plan)) != DC_OK) return rc;
+    if ((rc = pages_begin(ctx, stream, "kv8_fork", cache, &plan)) != DC_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if ((rc = dc_kv8_launch(ctx, "kv8_fork", fork_kernel, true, dim3(1), kPlanThreads, (cache->n_seqs + 31) / 32 * 4, s, *cache, src, dst, n, deep != 0, plan, ctx->status_dev)) != DC_OK)
         return rc;
@@ -518,7 +518,7 @@ extern "C" int dc_kv8_compact(dc_ctx* ctx, void* stream, const dc_kv8_cache* cac
     if (rc != DC_OK) return rc;
     const dc_device_scope scope(ctx);
     Plan plan;
-    if ((rc = pages_begin(ctx, "kv8_compact", cache, &plan)) != DC_OK) return rc;
+    if ((rc = pages_begin(ctx, stream, "kv8_compact", cache, &plan)) != DC_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if ((rc = dc_kv8_launch(ctx, "kv8_compact", compact_kernel, true, dim3(1), kPlanThreads, 0, s, *cache, plan, live)) != DC_OK) return rc;
     // at most half of the pages move

@@ -12,7 +12,7 @@
  *  - Pointers are device pointers already offset to the first element (the reference passes
  *    (buffer, byte offset) pairs). Dims and strides are in ELEMENTS, enums are uint32_t.
  *  - The caller owns every buffer. The context owns only its tensor-map cache, a status
- *    word and a bounded scratch workspace.
+ *    word, arrival counters and a bounded scratch workspace.
  *  - Return value 0 = DC_OK. Contract violations that the reference `assert!`s return
  *    DC_INVALID_ARG with a message readable through dc_last_error (latched, cleared on
  *    read), in the style of the reference's own C ABI (crates/decide-ane/src/lib.rs:22-35).
@@ -22,11 +22,11 @@
  *    buffers of the split GEMM and their arrival counters are one per context, so two streams
  *    running ops of one context concurrently race on them. Distinct contexts are independent.
  *  - Ops that need scratch (dc_attention with seq_start, dc_gated_delta, dc_conv_gated_delta,
- *    dc_convert_bf16_to_f16) take it from the context's workspace. If the workspace is too small
+ *    dc_convert_bf16_to_f16, dc_kv8_extend / _fork / _compact / _attention) take it from the context's workspace. If the workspace is too small
  *    the op grows it: a cudaFree + cudaMalloc, i.e. a device-wide synchronisation inside the
  *    call, which also fails under stream capture. To keep requests allocation-free, call
  *    dc_reserve_workspace once with the largest demand (dc_gated_delta_scratch_bytes,
- *    dc_attention_scratch_bytes), then dc_set_workspace_frozen(ctx, 1): from then on an op that
+ *    dc_attention_scratch_bytes, dc_kv8_*_scratch_bytes), then dc_set_workspace_frozen(ctx, 1): from then on an op that
  *    would have grown the workspace returns DC_INVALID_ARG instead. dc_model_* does both itself.
  */
 #ifndef DECIDE_CUDA_H
@@ -103,7 +103,7 @@ int dc_set_engine(dc_ctx* ctx, uint32_t family, uint32_t engine);
 /* Synchronises `stream`, then reports DC_TIMEOUT if a kernel's bounded wait ran out since the
  * last check (the analogue of the command-buffer status check, forward.rs:1022-1042), or
  * DC_INVALID_ARG if a kernel found a contract violation only it can see (dc_attention: a position at
- * or past the cache length given). */
+ * or past the cache length given; dc_kv8_*: what is said there). */
 int dc_check_status(dc_ctx* ctx, void* stream);
 /* Self-test of that path (no counterpart in the reference): enqueues one tiny kernel whose only
  * wait is on an mbarrier that nothing ever arrives at. The wait gives up at the library's limit
@@ -374,7 +374,9 @@ int dc_conv_gated_delta_supported(dc_ctx* ctx);
  *
  * What only the device can see (table, lens, refs, offsets, positions) is checked there: a violation raises the
  * status word, is reported by the next dc_check_status as DC_INVALID_ARG, and never reads or writes outside the
- * arrays described here. Unless an entry point says otherwise, what it concerns is skipped.
+ * arrays described here. Unless an entry point says otherwise, what it concerns is skipped. The calls can be captured into graphs
+ * once their scratch is reserved (a call that would allocate during a capture is DC_INVALID_ARG); a graph keeps the workspace that it
+ * was captured with, whatever later calls reserve.
  * ====================================================================================== */
 typedef struct dc_kv8_cache {
     void* k;                      /* e4m3 codes, 16-byte aligned; k and v have the same strides, in codes, multiples of 16: */
@@ -435,7 +437,7 @@ int dc_kv8_append(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t
  * (u32 [rows]), or with qpos NULL the sequence's rows are its last tokens. A row of DC_KV8_NO_KEYS, and every row of an empty
  * sequence, attends nothing: its output is zero. A position at or past lens[j] is a violation (the row attends all tokens there
  * are); a page id outside the pool makes the rows that attend it NaN. scale hd^-1/2, fp32 scores and softmax; the weights of the
- * V product are rounded to fp16 (they are at most 2^8 of the row's largest term). `gate` (fp32, row stride ldg, NULL = none)
+ * V product are rounded to fp16 (they are at most 2^8 of the row's largest term), those of few rows kept as two fp16 parts. `gate` (fp32, row stride ldg, NULL = none)
  * multiplies the output by sigmoid(gate). Writes rows below q_start[n_seqs] of y (the 16-bit type, row stride ldy), no others.
  * nq / nkv <= 16, max_q * nq / nkv < 2^28; q, y, gate 16-byte aligned, ldq, ldy multiples of 8, ldg of 4, each >= nq * hd. max_len: the longest
  * sequence, or more (it sizes the split of the keys; 0 = max_pages * page_size); a longer one is a violation. Scratch:

@@ -566,6 +566,48 @@ def test_another_stream_a_graph_and_a_frozen_workspace(k):
         k.dev.set_workspace_frozen(False)
 
 
+def test_a_graph_keeps_its_workspace(k):
+    """Scratch that grows after a capture, used by other calls in between, leaves the graph's own alone; a capture that would allocate is refused."""
+    from decide_b200.kernels import Device, Kernels
+    dev = Device(0)
+    fresh = Kernels(dev)
+    p = _filled(fresh, [2900, 10], 2, 128, 64)
+    nq, width = 8, 1024
+    q = torch.randn(2, width, device="cuda").to(dev.act_torch)
+    start = p.ints([0, 1, 2])
+    y, z = (torch.empty(2, width, dtype=dev.act_torch, device="cuda") for _ in range(2))
+    dev.reserve_workspace(p.ops.pages_scratch_bytes(p.gpu))
+    need = p.ops.attention_scratch_bytes(p.gpu, nq, 1, 2950)
+    assert need > dev.workspace_bytes
+
+    def attend(out):
+        p.ops.attention(None, p.gpu, 0, q, None, start, None, out, 2, width, 0, width, nq, 1, 2950)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q.mul_(1)
+        with pytest.raises(KernelError, match="during a capture"):
+            attend(y)
+    before = dev.workspace_bytes
+    dev.reserve_workspace(need)
+    assert dev.workspace_bytes == need > before
+    attend(z)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(y)
+    dev.reserve_workspace(need + (8 << 20))
+    filler = [torch.full((need // 4 + 64,), float("nan"), device="cuda") for _ in range(8)]   # what the old block's memory would hold by now
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        attend(z)
+        torch.cuda.synchronize()
+        assert torch.equal(y, z)
+    dev.check_status()
+    del graph, filler
+    dev.close()
+
+
 def test_follow_up_questions_share_a_state(k):
     """As they would be used: a request's state is written once, three questions fork it, each adds its rows and attends; one ends, the
     cache closes up, the others go on a token at a time and see what they saw before."""
