@@ -85,6 +85,28 @@ __device__ __forceinline__ uint64_t desc_mn128(uint32_t smem_addr, uint32_t atom
     return d;
 }
 
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 apart(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // 64 keys of a warp's 32 pairs: scores out of tensor memory, their maximum, then the weights into the columns that the scores came from.
 // MASKED: some pair of the warp does not see all 64 keys; `vis` of them it does. settled(): O may be rescaled.
 template <int HD, bool MASKED, typename F>
@@ -135,20 +157,21 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
         for (int g = 0; g < 2; ++g) {
             const uint32_t* v = s[h] + 16 * g;
             const float4 ab = sc[2 * h + g];
-            const float by = mul * ab.x, off = ab.y - m;
-            float sum0 = 0.f, sum1 = 0.f;
+            const uint64_t by = two(mul * ab.x, mul * ab.x), off = two(ab.y - m, ab.y - m);
+            uint64_t sums = two(0.f, 0.f);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                float p0 = ex2(fmaf(__uint_as_float(v[e]), by, off)), p1 = ex2(fmaf(__uint_as_float(v[e + 1]), by, off));
+                const float2 t = apart(fma_two(two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), by, off));
+                float p0 = ex2(t.x), p1 = ex2(t.y);
                 if (MASKED) {   // explicitly: a scale that is NaN, or a multiplier of zero, makes no zero of -infinity
                     p0 = 32 * h + 16 * g + e < vis ? p0 : 0.f;
                     p1 = 32 * h + 16 * g + e + 1 < vis ? p1 : 0.f;
                 }
                 w[8 * g + e / 2] = ActF16::pack(p0, p1);
-                sum0 += p0;   // (the total of the rounded weights, as kv8_attn.cu takes it, costs three instructions a weight: 300 -> 357 us
-                sum1 += p1;   // for 2,048 rows over 8,191 keys, and brings the error from 1.3 to 1.2 times that of rounding the output)
-            }
-            l = fmaf(sum0 + sum1, ab.z, l);
+                sums = add_two(sums, two(p0, p1));   // (the total of the rounded weights, as kv8_attn.cu takes it, costs three instructions a weight: 300 -> 357 us
+            }                                        // for 2,048 rows over 8,191 keys, and brings the error from 1.3 to 1.2 times that of rounding the output)
+            const float2 sum = apart(sums);
+            l = fmaf(sum.x + sum.y, ab.z, l);
         }
         tmem_st_32x32_x16(col_s + 16 * h, w);
     }
