@@ -18,9 +18,13 @@
 // both with one tile of 128 pairs (O has 256 columns) and stages of 64 keys; warps 5..7 then help the fillers, who have twice the codes for
 // each product (with three of them a half took 3,500 cycles).
 // Where there are fewer tiles than SMs the keys are cut into chunks, whose results a second kernel joins in chunk order.
-// Measured on the device, 32 query heads of 128 over 8 kv heads: 2,048 rows over 8,191 keys 300 us (800 TFLOP/s; tensor pipe 35 % busy, of 43 %
-// that 256 CTAs on 148 SMs allow), 178 rows over 2,491 keys 28 us; kv8_attn.cu takes 1,062 and 51. A round of both tiles' 64 keys takes
-// 2,050 cycles, its MMAs alone 1,250 (128x64x16 with both operands in shared memory 48 each, 128x128x16 with A in tensor memory 64).
+// Measured on the device, 32 query heads of 128 over 8 kv heads: 2,048 rows over 8,191 keys 288 us (833 TFLOP/s), 178 rows over 2,491 keys
+// 28 us; kv8_attn.cu takes 1,062 and 51. A round of both tiles' 64 keys takes about 2,000 cycles, its MMAs alone 1,250 (128x64x16 with both
+// operands in shared memory 48 each, 128x128x16 with A in tensor memory 64). What it is short of: without the softmax the same call takes
+// 241 us (one warp's issue of products; two warps 185), without its exponentials 266, without the fillers' work 259. Built and measured, and
+// slower for it: a warp of products for each tile and six fillers, 512 threads (301 us: the softmax of both tiles then runs in step and
+// shares the exponential units); the same with the tiles' exponentials in strict turns (308); fillers in a short loop of single groups
+// (299 to 336); fillers whose places are known to the compiler (543: the roles' code no longer fits the instruction cache).
 // Every wait is bounded; when one gives up the CTA raises the status word, waits for its products in flight and returns.
 #include "kv8_attn.cuh"
 #include "ptx.cuh"
@@ -85,8 +89,8 @@ __device__ __forceinline__ uint64_t desc_mn128(uint32_t smem_addr, uint32_t atom
     return d;
 }
 
-// Two fp32 operations an instruction.
-__device__ __forceinline__ uint64_t two(float lo, float hi) {
+// Two fp32 operations an instruction: 302 -> 288 us for 2,048 rows over 8,191 keys.
+__device__ __forceinline__ uint64_t side_by_side(float lo, float hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
     return r;
@@ -157,18 +161,18 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
         for (int g = 0; g < 2; ++g) {
             const uint32_t* v = s[h] + 16 * g;
             const float4 ab = sc[2 * h + g];
-            const uint64_t by = two(mul * ab.x, mul * ab.x), off = two(ab.y - m, ab.y - m);
-            uint64_t sums = two(0.f, 0.f);
+            const uint64_t by = side_by_side(mul * ab.x, mul * ab.x), off = side_by_side(ab.y - m, ab.y - m);
+            uint64_t sums = side_by_side(0.f, 0.f);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const float2 t = apart(fma_two(two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), by, off));
+                const float2 t = apart(fma_two(side_by_side(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), by, off));
                 float p0 = ex2(t.x), p1 = ex2(t.y);
                 if (MASKED) {   // explicitly: a scale that is NaN, or a multiplier of zero, makes no zero of -infinity
                     p0 = 32 * h + 16 * g + e < vis ? p0 : 0.f;
                     p1 = 32 * h + 16 * g + e + 1 < vis ? p1 : 0.f;
                 }
                 w[8 * g + e / 2] = ActF16::pack(p0, p1);
-                sums = add_two(sums, two(p0, p1));   // (the total of the rounded weights, as kv8_attn.cu takes it, costs three instructions a weight: 300 -> 357 us
+                sums = add_two(sums, side_by_side(p0, p1));   // (the total of the rounded weights, as kv8_attn.cu takes it, costs three instructions a weight: a fifth of the time
             }                                        // for 2,048 rows over 8,191 keys, and brings the error from 1.3 to 1.2 times that of rounding the output)
             const float2 sum = apart(sums);
             l = fmaf(sum.x + sum.y, ab.z, l);
@@ -483,11 +487,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                     }
                 }
             }
-            if (*abort_flag) {   // no product may still be writing tensor memory when it is freed
-                if (elect_one()) umma_commit(drain_bar);
-                __syncwarp();
-                mbar_wait(drain_bar, 0u, never_flag, a.status, 87);
-            }
         }
     } else {
         // -------------------------------------------------------------------------------- softmax: one thread per pair
@@ -626,6 +625,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 8) {
+        if (*abort_flag) {   // no product may still be writing tensor memory when it is freed
+            if (elect_one()) umma_commit(drain_bar);
+            __syncwarp();
+            mbar_wait(drain_bar, 0u, never_flag, a.status, 87);
+        }
         tc_fence_after_sync();
         __syncwarp();
         tmem_dealloc(tmem, kTmemCols);
