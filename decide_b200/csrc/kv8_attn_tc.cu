@@ -24,7 +24,8 @@
 // 241 us (one warp's issue of products; two warps 185), without its exponentials 266, without the fillers' work 259. Built and measured, and
 // slower for it: a warp of products for each tile and six fillers, 512 threads (301 us: the softmax of both tiles then runs in step and
 // shares the exponential units); the same with the tiles' exponentials in strict turns (308); scores of 128 keys in one product, which leaves
-// room for one buffer a tile (317, though the products alone take 198); fillers in a short loop of single groups (299 to 336); fillers whose places are known to the compiler (543: the roles' code no longer fits the instruction cache).
+// room for one buffer a tile (317, though the products alone take 198); fillers in a short loop of single groups (299 to 336); fillers
+// whose places are known to the compiler (543: the roles' code no longer fits the instruction cache).
 // Every wait is bounded; when one gives up the CTA raises the status word, waits for its products in flight and returns.
 #include "kv8_attn.cuh"
 #include "ptx.cuh"
