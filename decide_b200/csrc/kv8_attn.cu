@@ -2,10 +2,10 @@
 //
 // The mathematics. With codes k', v' and page scales a = 2^e_k, b = 2^e_v (per page and kv head), row r of head h has scores
 // s_j = a_j (q . k'_j) hd^-1/2 and o = sum_j softmax(s)_j b_j v'_j. Taking the V scale into the exponent, with t_j = s_j log2(e) + e_v(j):
-//     o = sum_j 2^(t_j - m) v'_j / sum_j 2^(t_j - m) 2^-e_v(j),    m any upper bound of t_j up to a factor,
+//     o = sum_j 2^(t_j - m) v'_j / sum_j 2^(t_j - m) 2^-e_v(j),    m the largest t_j up to a factor,
 // so that one running maximum serves both sums, the weights of the V product are relative to the row's largest TERM, and no code is
-// ever scaled: codes go into the tensor cores as fp16, exactly. The V product takes the weights in fp16 (relative to the row's largest
-// term they lose nothing that matters); the total is fp32.
+// ever scaled: codes go into the tensor cores as fp16, exactly. The V product takes the weights in fp16, whose range below the largest
+// term is what kKv8Below is about: a term under 2^-32 of it drops out of the product. The total is fp32.
 //
 // K/V bytes bound it when there are few rows. A CTA takes up to 8 NT (query row, head of the group) pairs that share a kv head's codes; its
 // warps take 16 keys each in turn with mma.sync m16n8k16, codes as the A operand (so that 16 keys, or 16 columns of V, fill it, and
@@ -69,8 +69,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 // A weight as the total counts it: rounded, as the V product takes it, so that what rounding does to a row that one key dominates cancels;
-// but exact where fp16 runs out of bits (below 2^-14 of the largest term), since a key whose page has a small V scale may weigh
-// much in the total and little in the product.
+// but exact where fp16 runs out of bits (below 2^-14), since a key whose page has a small V scale may weigh much in the total and
+// little in the product.
 __device__ __forceinline__ float kv8_total(float exact, float rounded) { return exact >= 6.103515625e-05f ? rounded : exact; }
 
 // One CTA: 8 NT (row, head) pairs of a sequence's kv head over one chunk of its keys.
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                     float top = fmaxf(s[b][e], s[b][2 + e]);
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(m[b][e], fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)));
+                    top = fmaxf(m[b][e], fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - kKv8Below);
                     const float by = ex2(m[b][e] - top);
                     m[b][e] = top;
                     l[b][e] *= by;
@@ -287,8 +287,8 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                     }
                 }
         }
-        // The weights as B fragments. One set of eight pairs goes in twice, rounded to fp16 and what that left (22 bits for eight more MMAs
-        // that memory hides); two sets go in once, and the total adds them as they go in (kv8_total).
+        // The weights as B fragments. One set of eight pairs goes in twice, rounded to fp16 and what that left (22 bits down to 2^-10 of the row's
+        // largest term, one less for each 2^-1 below, for eight more MMAs that memory hides); two sets go in once, and the total adds them as they go in (kv8_total).
         constexpr bool kTwice = NT == 1;
         uint32_t p0[NT], p1[NT], q0 = 0, q1 = 0;
 #pragma unroll

@@ -5,7 +5,11 @@
 namespace dc {
 
 constexpr float kKv8None = -1e30f;   // running maximum of a row that has seen nothing
-constexpr float kKv8Step = 8.0f;     // the maximum follows only when it grows by more than 2^8
+// Weights are 2^(t - m) in fp16, t a term's exponent. m is set to 2^7 below the largest term and follows it when that has grown by 2^8 more, so
+// that the largest weight is between 2^7 and 2^15: fp16's upper end. Its 11 bits then reach down to 2^-21 of the row's largest term and its last one to
+// 2^-31 (with m at the largest term itself, 2^-14 and 2^-24: beside a key of 2^26 times the weight all others were lost).
+constexpr float kKv8Below = 7.0f;
+constexpr float kKv8Step = kKv8Below + 8.0f;
 constexpr float kKv8Log2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {

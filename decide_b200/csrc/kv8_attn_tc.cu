@@ -139,9 +139,9 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
     const bool grow = top > m + kKv8Step;
     if (__any_sync(0xffffffffu, grow)) {
         // O and the total follow the new maximum (pairs whose maximum stays put scale by 1)
-        const float by = grow ? ex2(m - top) : 1.0f;
+        const float to = grow ? top - kKv8Below : m, by = ex2(m - to);
         l *= by;
-        if (grow) m = top;
+        m = to;
         if (scale_o) {
             if (!settled()) return false;
 #pragma unroll 1
@@ -172,9 +172,13 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
                     p0 = 32 * h + 16 * g + e < vis ? p0 : 0.f;
                     p1 = 32 * h + 16 * g + e + 1 < vis ? p1 : 0.f;
                 }
+                // cut to fp16's 11 bits, then exact in fp16 from 2^-14 on: product and total take the same weight, and what the cut does to all
+                // of a row's weights alike cancels (of weights rounded to nearest, as kv8_attn.cu has them, the total cost three instructions each)
+                p0 = __uint_as_float(__float_as_uint(p0) & 0xffffe000u);
+                p1 = __uint_as_float(__float_as_uint(p1) & 0xffffe000u);
                 w[8 * g + e / 2] = ActF16::pack(p0, p1);
-                sums = add_two(sums, side_by_side(p0, p1));   // (the total of the rounded weights, as kv8_attn.cu takes it, costs three instructions a weight: a fifth of the time
-            }                                        // for 2,048 rows over 8,191 keys, and brings the error from 1.3 to 1.2 times that of rounding the output)
+                sums = add_two(sums, side_by_side(p0, p1));
+            }
             const float2 sum = apart(sums);
             l = fmaf(sum.x + sum.y, ab.z, l);
         }

@@ -437,8 +437,10 @@ int dc_kv8_append(dc_ctx* ctx, void* stream, const dc_kv8_cache* cache, uint32_t
  * (u32 [rows]), or with qpos NULL the sequence's rows are its last tokens. A row of DC_KV8_NO_KEYS, and every row of an empty
  * sequence, attends nothing: its output is zero. A position at or past lens[j] is a violation (the row attends all tokens there
  * are); a page id outside the pool makes the rows that attend it NaN. scale hd^-1/2, fp32 scores and softmax; the weights of the
- * V product are rounded to fp16 (they are at most 2^8 of the row's largest term), those of few rows kept as two fp16 parts. `gate` (fp32, row stride ldg, NULL = none)
- * multiplies the output by sigmoid(gate). Writes rows below q_start[n_seqs] of y (the 16-bit type, row stride ldy), no others.
+ * V product are fp16: 11 bits (22 for few rows, as two fp16 parts) of a term weight * V scale down to 2^-21 (2^-10) of the row's largest such term, one less
+ * for each factor 2 below that, none under 2^-32; the scales of V that a row attends are at most 2^100 apart. `gate` (fp32, row
+ * stride ldg, NULL = none) multiplies the output by sigmoid(gate). Writes rows below q_start[n_seqs] of y (the 16-bit type, row
+ * stride ldy), no others.
  * nq / nkv <= 16, max_q * nq / nkv < 2^28; q, y, gate 16-byte aligned, ldq, ldy multiples of 8, ldg of 4, each >= nq * hd. max_len: the longest
  * sequence, or more (it sizes the split of the keys; 0 = max_pages * page_size); a longer one is a violation. Scratch:
  * dc_kv8_attention_scratch_bytes of the same nq, max_q and max_len. From 64 (row, head) pairs of a kv head in a sequence and enough

@@ -170,7 +170,7 @@ class Cache:
         s = np.repeat(scales[layer, ids, head], self.page)[:n]
         return c, s
 
-    def attention(self, layer, q, gate, q_start, qpos, half_step, bf16):
+    def attention(self, layer, q, gate, q_start, qpos, half_step, bf16, weight=2 * 2.0 ** -11, least=2.0 ** -25):
         """Returns (y, tolerance) [rows, nq * hd] in float64; NaN rows where a scale that is attended is NaN.
 
         The tolerance is what the kernel's arithmetic may be off by, term by term:
@@ -178,8 +178,8 @@ class Cache:
             and the argument of the exponential by 2^-22 of its size (in log2 units) twice;
           the exponential itself by 2^-22, each join of two partial sums by 2^-23 (32 of them are plenty), so a weight is off by a factor
             1 + w, and numerator and denominator each by as much;
-          weights in fp16: off by 2^-11 in the product, and in the total at most as much; those below 2^-14 of the row's largest term by 2^-25 of it in
-            absolute size in the product, and exact in the total;
+          weights in fp16: off by 2^-11 in the product, and in the total at most as much (`weight`: both together); small ones by `least` of the row's
+            largest term in absolute size in the product;
           bf16 queries: elements under 2^-28 of the row's largest are off by 2^-39 of it;
           the gate's sigmoid by 2^-20; the output by half a step of its type (`half_step` of its size; fp16 below 2^-14: 2^-25)."""
         rows, nq = q.shape[0], q.shape[1]
@@ -212,7 +212,7 @@ class Cache:
                     if bf16:
                         w += 2.0 ** -39 * np.abs(q[r, h]).max() * np.abs(k).sum(1).max() * hd ** -0.5
                     mass = p @ np.abs(v)
-                    t = (2 * w + 2 * 2.0 ** -11) * mass + 2.0 ** -25 * (p * vs[:see]).max() * np.abs(vc[:see]).sum(0)
+                    t = (2 * w + weight) * mass + least * (p * vs[:see]).max() * np.abs(vc[:see]).sum(0)
                     if gate is not None:
                         g = 1 / (1 + np.exp(-gate[r, cols]))
                         out, t = out * g, t * g + 2.0 ** -20 * np.abs(out) * g

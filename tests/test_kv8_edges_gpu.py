@@ -1,0 +1,109 @@
+"""The paged 8-bit K/V cache on the GPU at the ends of what its entry points allow: terms far below a row's largest, what a row does not
+attend, page bookkeeping that is wrong. Each case runs on the forms of the attention that it concerns: few rows, two sets of eight (row, head)
+pairs, whole tiles of the tensor cores. The numpy model and its tolerances are those of oracle/kv8.py."""
+import functools
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv8
+from tests.test_kv8_gpu import ROOM, Pair
+
+pytestmark = pytest.mark.gpu
+
+# What the weights of the V product may be off by, numerator and total together, and what a small one may be off by of the row's largest
+# term: two fp16 parts each take half of 2^-11 of what the one before left; 11 bits in both sums, 2^-10 apart at most. A row's largest
+# weight is at least 2^7, so that half a step of the smallest fp16 numbers, 2^-25, is 2^-32 of it.
+TWO_PARTS = dict(weight=2.0 ** -22, least=2.0 ** -32)
+ONE_PART = dict(weight=2 * 2.0 ** -11, least=2.0 ** -32)
+# rows that the last sequence brings, query heads and sequences for the three forms: up to eight pairs a tile, sixteen, 128 or 256
+FORMS = {"rows": dict(rows=1, nq=4, seqs=1), "pairs": dict(rows=5, nq=4, seqs=120), "tiles": dict(rows=33, nq=4, seqs=1)}
+
+
+def filled(k, form, n, hd, k_rows, v_rows, page=16):
+    """A cache whose last sequence holds n tokens with the K and V that k_rows(x), v_rows(x) make of normal numbers x [n, hd], written a page at a
+    time; the sequences before it hold one token each."""
+    f = FORMS[form]
+    p = Pair(k, n_pages=f["seqs"] - 1 + n // page + 2, nkv=1, hd=hd, n_seqs=f["seqs"], max_pages=max(n // page + 1, ROOM // page if form == "tiles" else 0), page=page)
+    p.model.attention = functools.partial(p.model.attention, **(TWO_PARTS if form == "rows" else ONE_PART))
+    counts = [1] * (f["seqs"] - 1) + [n]
+
+    def spoil(new):
+        for x, rows in zip(new, (k_rows, v_rows)):
+            at = len(x) - 2 - n
+            x[at:at + n, :hd] = rows(x[at:at + n, :hd].float()).to(x.dtype)
+    p.extend(counts)
+    p.append(counts, spoil=spoil)
+    return p, [1] * (f["seqs"] - 1) + [f["rows"]], f["nq"]
+
+
+def attend(p, form, counts, nq, **kw):
+    return p.attend(counts, nq, max_len=0 if form == "tiles" else None, **kw)
+
+
+# ---------------------------------------------------------------- terms far below the largest
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("gap", [12, 16, 20, 24, 26])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_key_that_takes_nearly_all_the_weight_hides_nothing(k, act, form, gap, hd):
+    """The first key weighs 2^gap as much as any other, and its V is zero: what is left is the others' V, 2^-gap of it each."""
+    n = 700
+
+    def k_rows(x):
+        x = x * 0.01
+        x[:, 0] = 0
+        x[0, 0] = gap * np.log(2) * hd ** 0.5 / 8
+        return x
+
+    def v_rows(x):
+        x = (x.abs() + 0.25) * 1024
+        x[0] = 0
+        return x
+    p, counts, nq = filled(k, form, n, hd, k_rows, v_rows)
+
+    def spoil(q):
+        q.mul_(0.01)
+        q.view(len(q), -1, hd)[:, :, 0] = 8
+    attend(p, form, counts, nq, gate=False, spoil=spoil)
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("gap", [8, 16, 18, 20])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_page_of_one_large_value_hides_nothing(k, act, form, gap, hd):
+    """One value of the first page raises the page's V scale to 2^gap times the others'; in the other columns that page's codes are zeros. All
+    keys behind it have one score, so that what their weights are rounded by does not average out. V is positive, so that errors are relative to the
+    sums: half a step of the output's type (2^-8 for bf16, 2^-11 for fp16), 2^-10 for weights of 11 bits in product and total, and 2^-14 for scores
+    below 1 (18 steps of 2^-22) and exponents below 2^5 (2^-21 of them, twice): together less than half a step and 2^-9."""
+    n = 700
+    size = 2.0 ** -10 if act == torch.float16 else 1.0
+
+    def k_rows(x):
+        x = x * 0
+        x[:16, 0] = 0.3 * hd ** 0.5 / 8
+        return x
+
+    def v_rows(x):
+        x = (x.abs() + 0.25).clamp(max=3.5) * size      # scales of 2^-7, the first page's 2^(gap - 7)
+        x[:16, 1:] = 0
+        x[3, 0] = 3.5 * size * 2.0 ** gap
+        return x
+    p, counts, nq = filled(k, form, n, hd, k_rows, v_rows)
+
+    def spoil(q):
+        q.mul_(0)
+        q.view(len(q), -1, hd)[:, :, 0] = 8
+    y = attend(p, form, counts, nq, gate=False, spoil=spoil)
+    q_rows, j = FORMS[form]["rows"], len(counts) - 1
+    got = y[j:j + q_rows, :nq * hd].double().cpu().numpy().reshape(q_rows, nq, hd)[:, :, 1:]
+    codes, scales = p.model.tokens(0, j, 0, p.model.v, p.model.v_scale)
+    key, key_scale = p.model.tokens(0, j, 0, p.model.k, p.model.k_scale)
+    weight = np.exp(key[:, 0] * key_scale * 8 / hd ** 0.5)
+    for i in range(q_rows):
+        see = n - q_rows + i + 1
+        want = weight[:see] @ (codes[:see] * scales[:see, None])[:, 1:] / weight[:see].sum()
+        assert (np.abs(got[i] - want) < (torch.finfo(act).eps / 2 + 2.0 ** -9) * want).all()
+    k.dev.check_status()
