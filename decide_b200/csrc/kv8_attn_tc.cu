@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         constexpr int kUnits = S::kUnits;
         constexpr uint32_t kRows = S::kRows, kPerGroup = 16 / kRows;   // keys of a unit, units of a group of 16 keys
         const int w = HD == 128 || warp < 8 ? (HD == 128 ? warp - 9 : warp - 5) : warp - 6, unit0 = 32 * w / S::kFillers, units = 32 * (w + 1) / S::kFillers - unit0;
-        const uint32_t token = static_cast<uint32_t>(a.c.token_stride), unit_step = kRows * token;
+        const uint32_t token = static_cast<uint32_t>(a.c.token_stride), unit_step = kRows * token;   // strides below 2^28: up to 15 of them fit 32 bits
         const uint32_t* table = a.c.table + static_cast<size_t>(j) * a.c.max_pages;
         // A lane's place in a unit: row bits from lane bits 2 and (of four rows) 4, 16-code piece c from bits 0, 1 and the others, so that the
         // eight lanes of a store's phase, four pieces of two rows, meet all 32 banks of the swizzled tile.
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                     kv8_flag(a.status, DC_STATUS_KV8_PAGE);
                     page[g] = 0;
                 }
-                at[g] = kc + page[g] * a.c.page_stride + (key & (a.c.page_size - 1)) * token;
+                at[g] = kc + page[g] * a.c.page_stride + (key & (a.c.page_size - 1)) * a.c.token_stride;   // 64 bits: up to 112 strides of 2^28
             }
         };
         uint4 kx[kUnits], vx[kUnits];

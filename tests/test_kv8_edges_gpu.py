@@ -107,3 +107,30 @@ def test_a_page_of_one_large_value_hides_nothing(k, act, form, gap, hd):
         want = weight[:see] @ (codes[:see] * scales[:see, None])[:, 1:] / weight[:see].sum()
         assert (np.abs(got[i] - want) < (torch.finfo(act).eps / 2 + 2.0 ** -9) * want).all()
     k.dev.check_status()
+
+
+# ---------------------------------------------------------------- strides
+
+@pytest.mark.parametrize("page,stride", [(128, 40_000_000), (64, 95_000_000)])
+def test_tokens_farther_apart_than_32_bits(k, page, stride):
+    """Tokens outermost: a page's last tokens lie more than 2^32 bytes behind its first. The same bits as from a cache that is contiguous."""
+    memory = torch.empty(page * stride, dtype=torch.uint8, device="cuda")
+    for hd in (128, 256):
+        n, rows, nq = 2 * page + page // 2 + 3, 33, 4
+        plain, far = (Pair(k, n_pages=5, nkv=1, hd=hd, n_seqs=1, max_pages=ROOM // page, page=page) for _ in range(2))
+        view = [memory.as_strided((1, 5, 1, page, hd), (0, hd, 0, stride, 1), at) for at in (0, 1 << 20)]
+        far.gpu = type(far.gpu)(*view, far.gpu.k_scale, far.gpu.v_scale, far.gpu.table, far.gpu.lens, far.gpu.refs)
+        y = []
+        for p in (plain, far):
+            p.extend([n])
+            p.append([n], seed=1)
+            y.append([p.attend([1], nq), p.attend([rows], nq, max_len=0)])
+        assert all(torch.equal(a, b) for a, b in zip(*y))
+        for name in ("k", "v"):
+            ids = plain.gpu.table[0, :3].long()
+            for i, q in enumerate(ids.tolist()):
+                held = min(page, n - i * page)
+                assert torch.equal(getattr(plain.gpu, name)[0, q, 0, :held], getattr(far.gpu, name)[0, q, 0, :held])
+    k.dev.check_status()
+    del memory, view, far, p
+    torch.cuda.empty_cache()
