@@ -205,7 +205,7 @@ extern "C" int dc_attention_rows(dc_ctx* ctx, void* stream, const void* q, const
     float* part = nullptr;
     if (slices > 1) {
         void* ws = nullptr;
-        if (int rc = dc_get_workspace(ctx, dc_attention_rows_scratch_bytes(ctx, rows, nq, nkv), "attention_rows", &ws); rc != DC_OK) return rc;
+        if (int rc = dc_stream_workspace(ctx, s, dc_attention_rows_scratch_bytes(ctx, rows, nq, nkv), "attention_rows", &ws); rc != DC_OK) return rc;
         part = static_cast<float*>(ws);
     }
     const bool f16 = ctx->act_dtype == DC_ACT_F16;

@@ -462,7 +462,7 @@ int dc_attention_tc(dc_ctx* ctx, cudaStream_t s, const void* q, const void* kc, 
     const uint32_t kv_rows = seq_start ? rows : kv_len, kv_max = seq_start ? max_len : kv_len;
     const uint32_t ldt = ((kv_rows + 7u) & ~7u) + 8u * n_seq;
     void* ws = nullptr;
-    int rc = dc_get_workspace(ctx, dc_attention_tc_scratch_bytes(kv_rows, n_seq, nkv), "attention", &ws);
+    int rc = dc_stream_workspace(ctx, s, dc_attention_tc_scratch_bytes(kv_rows, n_seq, nkv), "attention", &ws);
     if (rc != DC_OK) return rc;
     uint16_t* vt = static_cast<uint16_t*>(ws);
     CUtensorMap tq, tk, tv;

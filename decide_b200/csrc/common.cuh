@@ -12,6 +12,7 @@
 #include <map>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/decide_cuda.h"
 
@@ -24,7 +25,6 @@ typedef CUresult (*dc_encode_tiled_fn)(CUtensorMap*, CUtensorMapDataType, cuuint
 typedef std::tuple<const void*, uint32_t, uint32_t, uint32_t, uint32_t> dc_tmap_key;
 
 #define DC_KV8_DONE_COUNTERS 65536u
-#define DC_WORKSPACES_SET_ASIDE 16u
 
 struct dc_ctx {
     int device = 0;
@@ -50,8 +50,7 @@ struct dc_ctx {
     size_t workspace_bytes = 0;
     bool workspace_frozen = false;   // an op that needs more scratch than is reserved fails instead of allocating
     bool workspace_captured = false; // a captured graph holds the workspace: growing it sets it aside until dc_close
-    void* set_aside[DC_WORKSPACES_SET_ASIDE] = {};
-    uint32_t set_aside_count = 0;
+    std::vector<void*> set_aside;
     uint64_t allocs = 0;             // device/pinned allocations this context made (dc_open, workspace growth)
     uint64_t tmap_encodes = 0;       // tensor maps encoded (cache misses)
     void* tp_comm = nullptr;         // NCCL communicator of the tensor-parallel group (dc_tp_init), or null
@@ -59,14 +58,17 @@ struct dc_ctx {
     bool tp_exchange16 = false;      // partial sums cross the links in the 16-bit type (half the bytes) instead of fp32
 };
 
-
 int dc_fail(dc_ctx* ctx, int code, const char* fmt, ...);
 int dc_check_launch(dc_ctx* ctx, const char* what);
-// Hands out the context's scratch workspace, at least `bytes` long, in *out. Growing it frees and
+// Makes the context's scratch workspace at least `bytes` long and hands it out in *out. Growing it frees and
 // allocates device memory (a device-wide synchronisation): callers that must not allocate inside a
 // request reserve up front (dc_reserve_workspace) and freeze it (dc_set_workspace_frozen), after
-// which a larger demand is DC_INVALID_ARG naming `who`.
+// which a larger demand is DC_INVALID_ARG naming `who`. A workspace that a captured graph was given stays allocated until
+// dc_close: growing sets it aside.
 int dc_get_workspace(dc_ctx* ctx, size_t bytes, const char* who, void** out);
+// The same for an op that enqueues on `stream`, which every op uses: notes where a capture is what asks, and refuses a
+// capture that would have to allocate before it breaks.
+int dc_stream_workspace(dc_ctx* ctx, cudaStream_t stream, size_t bytes, const char* who, void** out);
 // One-time per-device kernel set-up of each family (opt-in shared-memory sizes): what dc_warm_up runs.
 int dc_gemm_warm(dc_ctx* ctx);
 int dc_attention_warm(dc_ctx* ctx);

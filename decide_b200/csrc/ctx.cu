@@ -34,10 +34,7 @@ int dc_get_workspace(dc_ctx* ctx, size_t bytes, const char* who, void** out) {
         return dc_fail(ctx, DC_INVALID_ARG, "%s: needs %zu bytes of scratch but the workspace is frozen at %zu (reserve more with dc_reserve_workspace before freezing)",
                        who, bytes, ctx->workspace_bytes);
     if (ctx->workspace_captured) {
-        if (ctx->set_aside_count == DC_WORKSPACES_SET_ASIDE)
-            return dc_fail(ctx, DC_INVALID_ARG, "%s: needs %zu bytes of scratch, and the workspace has grown %u times under captured graphs already (reserve more with dc_reserve_workspace)",
-                           who, bytes, DC_WORKSPACES_SET_ASIDE);
-        ctx->set_aside[ctx->set_aside_count++] = ctx->workspace;
+        ctx->set_aside.push_back(ctx->workspace);
         ctx->workspace_captured = false;
     } else if (ctx->workspace) {
         cudaFree(ctx->workspace);
@@ -56,7 +53,7 @@ int dc_get_workspace(dc_ctx* ctx, size_t bytes, const char* who, void** out) {
     return DC_OK;
 }
 
-int dc_kv8_workspace(dc_ctx* ctx, cudaStream_t stream, size_t bytes, const char* who, void** out) {
+int dc_stream_workspace(dc_ctx* ctx, cudaStream_t stream, size_t bytes, const char* who, void** out) {
     cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(stream, &state) != cudaSuccess) cudaGetLastError();   // the default stream while another one captures
     const bool captured = state == cudaStreamCaptureStatusActive;
@@ -191,7 +188,7 @@ void dc_close(dc_ctx* ctx) {
     if (ctx->status_dev) cudaFree(ctx->status_dev);
     if (ctx->status_host) cudaFreeHost(ctx->status_host);
     if (ctx->workspace) cudaFree(ctx->workspace);
-    for (uint32_t i = 0; i < ctx->set_aside_count; ++i) cudaFree(ctx->set_aside[i]);
+    for (void* p : ctx->set_aside) cudaFree(p);
     if (ctx->kv8_done) cudaFree(ctx->kv8_done);
     if (ctx->gemm_part_ws) cudaFree(ctx->gemm_part_ws);
     if (ctx->gemm_part_cnt) cudaFree(ctx->gemm_part_cnt);

@@ -1375,7 +1375,7 @@ int dc_gated_delta_chunked(dc_ctx* ctx, cudaStream_t s, const float* q, const fl
         return dc_fail(ctx, DC_UNSUPPORTED, "conv_gated_delta: the fused form exists for the tcgen05 engine with split 3 only");
     const size_t bytes = dc_delta_chunk_scratch_bytes(t, n_seq, nv);
     void* ws = nullptr;
-    if (int rc = dc_get_workspace(ctx, bytes, "gated_delta", &ws); rc != DC_OK) return rc;
+    if (int rc = dc_stream_workspace(ctx, s, bytes, "gated_delta", &ws); rc != DC_OK) return rc;
     args.scratch = static_cast<uint8_t*>(ws);
     const uint32_t max_chunks = (max_len + C - 1) / C;
     if (split == 1) return launch_chunked<1>(ctx, s, args, n_seq, max_chunks);

@@ -17,10 +17,6 @@ enum {
 // Host-side checks of a call: DC_OK, or dc_fail with `who` in the message.
 int dc_kv8_require(dc_ctx* ctx, const char* who, const dc_kv8_cache* cache);
 
-// Scratch of a call: dc_get_workspace, but a captured graph that was given the workspace keeps it (a later call that needs more leaves it
-// allocated until dc_close), and a capture that would have to allocate is refused before it breaks.
-int dc_kv8_workspace(dc_ctx* ctx, cudaStream_t stream, size_t bytes, const char* who, void** out);
-
 int dc_kv8_attention_warm(dc_ctx* ctx);
 int dc_kv8_attention_tc_warm(dc_ctx* ctx);
 

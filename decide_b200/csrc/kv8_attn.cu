@@ -572,7 +572,7 @@ extern "C" int dc_kv8_attention(dc_ctx* ctx, void* stream, const dc_kv8_cache* c
     a.done = ctx->kv8_done;
     if (t.chunks > 1) {
         void* ws = nullptr;
-        if ((rc = dc_kv8_workspace(ctx, static_cast<cudaStream_t>(stream), t.part_bytes, "kv8_attention", &ws)) != DC_OK) return rc;
+        if ((rc = dc_stream_workspace(ctx, static_cast<cudaStream_t>(stream), t.part_bytes, "kv8_attention", &ws)) != DC_OK) return rc;
         a.part = static_cast<float*>(ws);
     }
     if ((rc = dc_kv8_attention_warm(ctx)) != DC_OK) return rc;

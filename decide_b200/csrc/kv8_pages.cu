@@ -416,7 +416,7 @@ uint32_t copy_grid(const dc_ctx* ctx, const dc_kv8_cache* c, uint64_t moves) {
 
 int pages_begin(dc_ctx* ctx, void* stream, const char* who, const dc_kv8_cache* cache, Plan* plan) {
     void* ws = nullptr;
-    const int rc = dc_kv8_workspace(ctx, static_cast<cudaStream_t>(stream), plan_bytes(cache->n_pages), who, &ws);
+    const int rc = dc_stream_workspace(ctx, static_cast<cudaStream_t>(stream), plan_bytes(cache->n_pages), who, &ws);
     if (rc == DC_OK) *plan = plan_at(ws, cache->n_pages);
     return rc;
 }

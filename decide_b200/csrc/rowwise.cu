@@ -283,7 +283,7 @@ int dc_convert_bf16_to_f16(dc_ctx* ctx, void* stream, const void* src, void* dst
     DC_REQUIRE(ctx, src && dst, "convert: null operand");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     void* ws = nullptr;
-    if (int rc = dc_get_workspace(ctx, 64, "convert", &ws); rc != DC_OK) return rc;
+    if (int rc = dc_stream_workspace(ctx, s, 64, "convert", &ws); rc != DC_OK) return rc;
     unsigned long long* counters = static_cast<unsigned long long*>(ws);
     cudaError_t e = cudaMemsetAsync(counters, 0, 32, s);
     if (e != cudaSuccess) return dc_fail(ctx, DC_CUDA_ERROR, "convert: %s", cudaGetErrorString(e));

@@ -24,10 +24,11 @@
  *  - Ops that need scratch (dc_attention with seq_start, dc_gated_delta, dc_conv_gated_delta,
  *    dc_convert_bf16_to_f16, dc_kv8_extend / _fork / _compact / _attention) take it from the context's workspace. If the workspace is too small
  *    the op grows it: a cudaFree + cudaMalloc, i.e. a device-wide synchronisation inside the
- *    call, which also fails under stream capture. To keep requests allocation-free, call
+ *    call; under stream capture the call is DC_INVALID_ARG instead. A graph keeps the workspace that it was captured with
+ *    (the caller's, or dc_model_*'s own): growing then leaves that block allocated until dc_close. To keep requests allocation-free, call
  *    dc_reserve_workspace once with the largest demand (dc_gated_delta_scratch_bytes,
  *    dc_attention_scratch_bytes, dc_kv8_*_scratch_bytes), then dc_set_workspace_frozen(ctx, 1): from then on an op that
- *    would have grown the workspace returns DC_INVALID_ARG instead. dc_model_* does both itself.
+ *    would have grown the workspace returns DC_INVALID_ARG instead. dc_model_* reserves what its forwards need when it is created, and none grows the workspace.
  */
 #ifndef DECIDE_CUDA_H
 #define DECIDE_CUDA_H
