@@ -20,8 +20,8 @@
 // 16-byte pieces of each 128 bytes of a row lie at piece ^ 4 (row & 1) for K and piece ^ (row & 6) for V: a row is written in
 // one pass over the banks, and the eight lanes of a read's phase, two keys by four pieces of K or four keys by two of V, meet all 32
 // banks. (Pieces lying where their lanes read them were written four passes a row: 201 instead of 68 a tile, which bound the kernel.)
-// Codes that append has written are finite; what lies behind a sequence's last token may be the code for NaN, and a weight of zero
-// would not hide it: those V codes are replaced by zeros.
+// Codes that append has written are finite; what lies behind a sequence's last token, or has not been written since the sequence
+// grew, may be the code for NaN, and a weight of zero would not hide it: V codes that no row of the tile attends are replaced by zeros.
 // Keys are cut into chunks over CTAs; partial results meet in the workspace, and the CTA of a tile that finishes last (a counter tells)
 // joins them in chunk order, so that the result does not depend on timing.
 // Measured on the device, 8 kv heads of 128, 4 queries each: one token over 131,071 keys 51 us (268 MB, 5.3 TB/s); a token for each of 64
@@ -315,10 +315,10 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                 const uint4 u = *reinterpret_cast<const uint4*>(at + read_v + ((p & 1) + 8 * (p >> 1)) * HD + 128 * v);
                 x[p][0] = u.x, x[p][1] = u.y, x[p][2] = u.z, x[p][3] = u.w;
             }
-            if (key + kTile > r.len) {   // what lies behind the last token
+            if (key + kTile > most) {   // what no row of the tile attends
 #pragma unroll
                 for (int p = 0; p < 4; ++p)
-                    if (key + 2 * t + (p & 1) + 8 * (p >> 1) >= r.len) x[p][0] = x[p][1] = x[p][2] = x[p][3] = 0u;
+                    if (key + 2 * t + (p & 1) + 8 * (p >> 1) >= most) x[p][0] = x[p][1] = x[p][2] = x[p][3] = 0u;
             }
 #pragma unroll
             for (int d = 0; d < 8; ++d) {   // columns 2 d and 2 d + 1 of the lane's 16

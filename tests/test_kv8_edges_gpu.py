@@ -134,3 +134,47 @@ def test_tokens_farther_apart_than_32_bits(k, page, stride):
     k.dev.check_status()
     del memory, view, far, p
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------- what a row does not attend
+
+def spread(k, form, hd, spare=0):
+    """The form's last sequence over 300 tokens, with rows at the places `at`; pages 0 and 1 are free and hold the codes for NaN. `spare` tokens more are
+    its own but not written."""
+    f = FORMS[form]
+    rows, n = max(f["rows"], 2), 300
+    p = Pair(k, n_pages=f["seqs"] + n // 16 + spare // 16 + 6, nkv=2, hd=hd, n_seqs=f["seqs"] + 1, max_pages=ROOM // 16 if form == "tiles" else 30, page=16)
+    p.extend([20] + [1] * (f["seqs"] - 1) + [0])
+    p.append([20] + [1] * (f["seqs"] - 1) + [0])
+    p.extend([0] * f["seqs"] + [n])
+    p.append([0] * f["seqs"] + [n], seed=1)
+    p.free([0])
+    p.gpu.k[:, :2], p.gpu.v[:, :2], p.model.k[:, :2], p.model.v[:, :2] = 0x7F, 0x7F, 0x7F, 0x7F
+    if spare:
+        p.extend([0] * f["seqs"] + [spare])
+    at = [(i * 23 + 3) % 60 for i in range(rows)]       # within the first four pages
+    return p, [0] + [1] * (f["seqs"] - 1) + [rows], [0] * (f["seqs"] - 1) + at, f["nq"]
+
+
+def call(p, counts, nq, qpos, seed=5):
+    """The attention call as it is, without the model: outputs [rows, nq * hd] in float64."""
+    start, hd, act = np.concatenate([[0], np.cumsum(counts)]), p.gpu.hd, p.dev.act_torch
+    rows, width = int(start[-1]), nq * hd
+    q = torch.randn(rows, width, generator=torch.Generator().manual_seed(seed)).to(act)
+    y = torch.full((rows, width), 7.0, dtype=act, device="cuda")
+    p.ops.attention(None, p.gpu, 0, q.cuda(), None, p.ints(start), p.ints(qpos), y, rows, width, 0, width, nq, max(counts), 0)
+    want, tol = p.model.attention(0, q.double().numpy().reshape(rows, nq, hd), None, start, np.array(qpos), torch.finfo(act).eps / 2, act == torch.bfloat16)
+    return y.double().cpu().numpy(), want, tol
+
+
+@pytest.mark.parametrize("spare", [1, 4, 40])
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_tokens_that_are_not_written_yet_reach_no_row(k, act, form, hd, spare):
+    """A sequence that has been lengthened but not written to: its memory holds the codes for NaN, its new pages' scales are NaN. Rows that see all the
+    written tokens, in the middle of a page, and rows that see few."""
+    p, counts, qpos, nq = spread(k, form, hd, spare)
+    qpos[-1] = 299
+    got, want, tol = call(p, counts, nq, qpos)
+    assert (np.abs(got - want) <= tol).all()
+    k.dev.check_status()
