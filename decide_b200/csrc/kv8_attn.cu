@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
             page_at = page * a.c.page_stride + kvh * a.c.head_stride + (key & (a.c.page_size - 1)) * a.c.token_stride;
             next_k = a.c.k_scale[static_cast<size_t>(page) * a.c.nkv + kvh];
             next_v = a.c.v_scale[static_cast<size_t>(page) * a.c.nkv + kvh];
-            if (!inside) next_k = __uint_as_float(0x7fffffffu);   // what attends it is NaN
+            if (!inside) next_k = __uint_as_float(0x7fffffffu);   // what attends it is NaN (and page 0's V codes are not used)
         }
     };
 
@@ -315,10 +315,10 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                 const uint4 u = *reinterpret_cast<const uint4*>(at + read_v + ((p & 1) + 8 * (p >> 1)) * HD + 128 * v);
                 x[p][0] = u.x, x[p][1] = u.y, x[p][2] = u.z, x[p][3] = u.w;
             }
-            if (key + kTile > most) {   // what no row of the tile attends
+            if (key + kTile > most || isnan(ks)) {   // what no row of the tile attends; what stands in for a page that is not there
 #pragma unroll
                 for (int p = 0; p < 4; ++p)
-                    if (key + 2 * t + (p & 1) + 8 * (p >> 1) >= most) x[p][0] = x[p][1] = x[p][2] = x[p][3] = 0u;
+                    if (key + 2 * t + (p & 1) + 8 * (p >> 1) >= most || isnan(ks)) x[p][0] = x[p][1] = x[p][2] = x[p][3] = 0u;
             }
 #pragma unroll
             for (int d = 0; d < 8; ++d) {   // columns 2 d and 2 d + 1 of the lane's 16

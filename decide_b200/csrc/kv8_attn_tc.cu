@@ -312,13 +312,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             }
         };
         const uint8_t* at[kGroups];   // first code of the group in K, this lane's; V lies at the same distance from its first
+        // What stands in for a page outside the pool has to hold numbers, or pairs that do not attend it would take the code for NaN times a weight of
+        // zero: the sequence's first page, which is full where a later one is attended. Where the first is itself outside the pool every
+        // pair that attends anything is NaN. (Zeros instead, chosen at each load, took 12 % of the time of 2,048 rows over 8,191 keys.)
         auto to_page = [&](uint32_t step) {
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
                 const uint32_t key = key0 + step * kKeys + 16 * (group0 + g);
                 if (page[g] >= a.c.n_pages) {
                     kv8_flag(a.status, DC_STATUS_KV8_PAGE);
-                    page[g] = 0;
+                    page[g] = __ldg(table);
+                    if (page[g] >= a.c.n_pages) page[g] = 0;
                 }
                 at[g] = kc + page[g] * a.c.page_stride + (key & (a.c.page_size - 1)) * a.c.token_stride;   // 64 bits: up to 112 strides of 2^28
             }
@@ -554,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         }
         // the divisor, for whoever stores the pair's columns
         if (HD == 256 && x == 0 && ok && !idle) {
-            rank[p] = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+            rank[p] = l == 0.f ? 0.f : whole ? 1.0f / l : 1.0f;
             __syncwarp();
             if (lane == 0) mbar_arrive(l_full);
         }
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             __syncwarp();
             tc_fence_after_sync();
             uint8_t* stage = smem + S::kQ + warp * 8192;
-            const float by = HD == 256 ? rank[first + lane] : whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+            const float by = HD == 256 ? rank[first + lane] : l == 0.f ? 0.f : whole ? 1.0f / l : 1.0f;   // 0: the pair attends nothing here, whatever lies in O
             const uint32_t col8 = lane & 7, col_o = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColO + 128 * (x + part);   // eight lanes a row
             float* parts = a.part + (static_cast<size_t>(tile_id) * a.chunks + z) * kPairs * kLd;
             if (!whole && part == 0 && first + lane < here) *reinterpret_cast<float2*>(parts + (first + lane) * kLd + HD) = make_float2(m, l);
@@ -600,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         uint4 o = make_uint4(0, 0, 0, 0);
-                        if (halves) o = make_uint4(__float_as_uint(__uint_as_float(v[e]) * by), __float_as_uint(__uint_as_float(v[e + 1]) * by),
+                        if (halves && by != 0.f) o = make_uint4(__float_as_uint(__uint_as_float(v[e]) * by), __float_as_uint(__uint_as_float(v[e + 1]) * by),
                                                    __float_as_uint(__uint_as_float(v[e + 2]) * by), __float_as_uint(__uint_as_float(v[e + 3]) * by));
                         *reinterpret_cast<uint4*>(stage + lane * 256 + (((4 * q4 + e / 4) ^ (lane & 15)) << 4)) = o;
                     }

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+from decide_b200.kernels import KernelError
 from oracle import kv8
 from tests.test_kv8_gpu import ROOM, Pair
 
@@ -178,3 +179,33 @@ def test_tokens_that_are_not_written_yet_reach_no_row(k, act, form, hd, spare):
     got, want, tol = call(p, counts, nq, qpos)
     assert (np.abs(got - want) <= tol).all()
     k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_bad_page_reaches_the_rows_that_attend_it_alone(k, act, form, hd):
+    p, counts, qpos, nq = spread(k, form, hd)
+    last = len(qpos) - 1
+    qpos[last] = 299                                        # attends the page that is spoilt below; the others do not
+    j = len(counts) - 1
+    first = last - counts[j] + 1                            # the sequence's first row
+    for bad in (p.gpu.n_pages, -1):
+        for column in (6, 18):                              # in the middle, and where the sequence ends
+            good = int(p.gpu.table[j, column])
+            p.gpu.table[j, column] = bad
+            got, want, tol = call(p, counts, nq, qpos)
+            p.gpu.table[j, column] = good
+            assert np.isnan(got[last]).all()
+            assert (np.abs(got[:last] - want[:last]) <= tol[:last]).all()
+            with pytest.raises(KernelError, match="outside the pool"):
+                k.dev.check_status()
+    got, want, tol = call(p, counts, nq, qpos)
+    assert (np.abs(got - want) <= tol).all()
+    k.dev.check_status()
+    # the first page: all that attend anything are NaN, a row that attends nothing is zero
+    qpos[first] = kv8.NO_KEYS
+    p.gpu.table[j, 0] = p.gpu.n_pages
+    got, want, tol = call(p, counts, nq, qpos)
+    assert (got[first] == 0).all() and np.isnan(got[first + 1:]).all() and (np.abs(got[:first] - want[:first]) <= tol[:first]).all()
+    with pytest.raises(KernelError, match="outside the pool"):
+        k.dev.check_status()
