@@ -344,16 +344,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         };
         // filler 0 also keeps the scales of the stage's groups, lane g those of group g
         uint32_t scale_page = 0;
+        bool scale_there = false;   // the group has a key that some pair attends: others have no page whose scale means anything
         float k_scale = 0.f, v_scale = 1.f;
         auto scale_look_up = [&](uint32_t step) {
             const uint32_t key = key0 + step * kKeys + 16 * (lane % S::kGroups);
-            scale_page = key < key1 ? __ldg(table + (key >> a.page_shift)) : 0u;
+            scale_there = key < key1;
+            scale_page = scale_there ? __ldg(table + (key >> a.page_shift)) : 0u;
         };
         auto scale_load = [&] {
             const size_t s = static_cast<size_t>(scale_page < a.c.n_pages ? scale_page : 0u) * a.c.nkv + kvh;
             k_scale = a.c.k_scale[s];
             v_scale = a.c.v_scale[s];
             if (scale_page >= a.c.n_pages) k_scale = __uint_as_float(0x7fffffffu);   // what attends it is NaN
+            if (!scale_there) k_scale = v_scale = 1.f;
         };
         // 16 codes become the 16-byte pieces 2 c and 2 c + 1 of the row, eight pieces to an atom, at piece ^ (row % 8): with row = kRows u + fr that
         // is one address and its neighbour at ^ 16, both at ^ 16 (kRows u % 8)

@@ -209,3 +209,17 @@ def test_a_bad_page_reaches_the_rows_that_attend_it_alone(k, act, form, hd):
     assert (got[first] == 0).all() and np.isnan(got[first + 1:]).all() and (np.abs(got[:first] - want[:first]) <= tol[:first]).all()
     with pytest.raises(KernelError, match="outside the pool"):
         k.dev.check_status()
+
+
+@pytest.mark.parametrize("scale", [-3.0, 0.0, float("inf"), float("nan")])
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_of_pages_nobody_holds_are_not_used(k, act, form, hd, scale):
+    """Keys are taken sixteen, and scores 64, at a time: what lies past the last key that any row attends has no page."""
+    p, counts, qpos, nq = spread(k, form, hd)
+    qpos = [i % 40 for i in qpos]
+    for s in (p.gpu.k_scale, p.gpu.v_scale):
+        s[:, :2] = scale
+    got, want, tol = call(p, counts, nq, qpos)
+    assert (np.abs(got - want) <= tol).all()
+    k.dev.check_status()
