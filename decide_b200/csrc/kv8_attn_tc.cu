@@ -70,6 +70,12 @@ __device__ __forceinline__ void sts16(uint32_t to, uint32_t x, uint32_t y, uint3
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// A bounded wait of a whole warp: its lanes agree on whether it is over. Of lanes that saw the limit pass and lanes that saw the phase complete some
+// would leave for the CTA's barrier and the others stay at the next instruction of the whole warp, for good.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
+}
+
 // Advances a two-stage ring.
 struct Ring {
     uint32_t stage = 0, phase = 0;
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             look_up(1);
         }
         for (uint32_t i = 0; i < steps; ++i) {
-            if (i >= 2 && !(ok = mbar_wait(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81))) break;
+            if (i >= 2 && !(ok = warp_wait(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81))) break;
             if (w == 0 && lane < S::kGroups) {
                 const float e = kv8_log2i(v_scale);   // a NaN reaches the total through the weights, not through 1 / V scale
                 scales[(i % kScaleSlots) * 8 + lane] = make_float4(k_scale, e, isnan(e) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(e)))), 0.f);
@@ -402,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                 to_page(i + 1);
                 load(kx, 0, i + 1);
             }
-            if (i >= 2 && !(ok = mbar_wait(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82))) break;
+            if (i >= 2 && !(ok = warp_wait(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82))) break;
             store(vx, S::kV + ring.stage * S::kStage);
             fence_proxy_async_smem();
             __syncwarp();
@@ -430,8 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             const uint32_t n = halves;
             const bool both = two;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-                const bool done = mbar_wait(bar, parity, abort_flag, a.status, code);
-                return __all_sync(0xffffffffu, done);
+                return warp_wait(bar, parity, abort_flag, a.status, code);
             };
             // half u of a round of four: buffer u % 2; `last`: the stage's last product of the kind
             auto scores = [&](int x, int u, bool last) {
@@ -538,15 +543,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         const uint32_t see = on ? seen[p] : most;    // pairs past the last are computed (their q is zero) and not stored
         for (uint32_t h = 0; runs && ok && h < halves; ++h) {
             const uint32_t step = h / S::kHalves;
-            if (!(ok = mbar_wait(&scale_full[step % kScaleSlots], step / kScaleSlots & 1u, abort_flag, a.status, 88))) break;
-            if (!(ok = mbar_wait(&s_full[2 * x + (h & 1)], h >> 1 & 1, abort_flag, a.status, 89))) break;
+            if (!(ok = warp_wait(&scale_full[step % kScaleSlots], step / kScaleSlots & 1u, abort_flag, a.status, 88))) break;
+            if (!(ok = warp_wait(&s_full[2 * x + (h & 1)], h >> 1 & 1, abort_flag, a.status, 89))) break;
             __syncwarp();
             tc_fence_after_sync();
             const float4* sc = scales + step % kScaleSlots * 8 + 4 * (h % S::kHalves);
             const uint32_t key = key0 + h * kHalf, col_s = lanes + 128 * x + 64 * (h & 1);
             const int vis = static_cast<int>(min(see, key + kHalf)) - static_cast<int>(min(see, key));   // of the 64 keys
             auto settled = [&] {   // the V product of the last 64 keys: the one before it came before these scores, the next has no weights yet
-                const bool done = mbar_wait(&pv_done[x], (h - 1) & 1u, abort_flag, a.status, 91);
+                const bool done = warp_wait(&pv_done[x], (h - 1) & 1u, abort_flag, a.status, 91);
                 __syncwarp();
                 tc_fence_after_sync();
                 return done;
@@ -575,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     if (warp < 8 && ok && !idle && (HD == 256 || warp < 4 || two)) {
         const uint32_t x = HD == 256 ? 0 : warp >> 2, part = HD == 256 ? warp >> 2 : 0, first = HD == 256 ? 32 * (warp & 3) : 32 * warp;   // tile, 128 columns, pair of lane 0
         // (pv_done cannot tell: it may have run two phases ahead, and a wait for a phase that lies two back waits for the next one like it)
-        const bool there = (HD == 128 || mbar_wait(l_full, 0u, abort_flag, a.status, 92)) && (halves == 0 || mbar_wait(&o_full[x], 0u, abort_flag, a.status, 90));
+        const bool there = (HD == 128 || warp_wait(l_full, 0u, abort_flag, a.status, 92)) && (halves == 0 || warp_wait(&o_full[x], 0u, abort_flag, a.status, 90));
         if (there) {
             __syncwarp();
             tc_fence_after_sync();
