@@ -284,7 +284,11 @@ __global__ void __launch_bounds__(128) free_kernel(dc_kv8_cache c, const uint32_
         const uint32_t page = c.table[static_cast<size_t>(j) * c.max_pages + col];
         if (page >= c.n_pages) {
             kv8_flag(status, DC_STATUS_KV8_PAGE);
-        } else if (atomicSub(&c.refs[page], 1u) == 0u) {
+            continue;
+        }
+        // Several sequences of the call may name a page that fewer hold. Whoever finds none left, or fewer than none while another is about to put
+        // its own back, puts it back: none does so before all that were held are gone, so the count ends at zero.
+        if (static_cast<int>(atomicSub(&c.refs[page], 1u)) <= 0) {
             atomicAdd(&c.refs[page], 1u);
             kv8_flag(status, DC_STATUS_KV8_REFS);
         }

@@ -223,3 +223,24 @@ def test_scales_of_pages_nobody_holds_are_not_used(k, act, form, hd, scale):
     got, want, tol = call(p, counts, nq, qpos)
     assert (np.abs(got - want) <= tol).all()
     k.dev.check_status()
+
+
+# ---------------------------------------------------------------- pages that are wrong
+
+def test_a_page_freed_too_often_ends_at_none(k):
+    """Two hundred sequences that all name one page, of which the counts know fewer, freed in one call: no count falls below zero."""
+    for holders in (0, 1, 3, 199, 200):
+        for _ in range(10):
+            p = Pair(k, n_pages=300, nkv=1, n_seqs=200, max_pages=2, page=16)
+            p.extend([20] * 100 + [0] * 100)
+            p.gpu.lens[100:] = 3
+            p.gpu.table[:, 0] = 250
+            p.gpu.refs[250] = holders
+            p.ops.free(None, p.gpu, p.ints(range(200)), 200)
+            assert int(p.gpu.refs[250]) == 0 and p.gpu.lens.tolist() == [0] * 200
+            assert int(p.gpu.refs.sum()) == 100         # what the table no longer names
+            if holders < 200:
+                with pytest.raises(KernelError, match="freed more often"):
+                    k.dev.check_status()
+            else:
+                k.dev.check_status()
