@@ -244,3 +244,201 @@ def test_a_page_freed_too_often_ends_at_none(k):
                     k.dev.check_status()
             else:
                 k.dev.check_status()
+
+
+# ---------------------------------------------------------------- the forms on inputs that are not easy
+
+def grown(k, form, hd, sizes, page=16, nkv=2, layers=1, spoil=None, bits=True):
+    """The form's last sequence, written a page at a time with K and V of the sizes given; the ones before it hold 7 tokens."""
+    f = FORMS[form]
+    n = page * len(sizes)
+    p = Pair(k, layers=layers, n_pages=f["seqs"] - 1 + len(sizes) + 3, nkv=nkv, hd=hd, n_seqs=f["seqs"], max_pages=max(len(sizes) + 1, ROOM // page if form == "tiles" else 0), page=page)
+    if bits:
+        p.model.attention = functools.partial(p.model.attention, **(TWO_PARTS if form == "rows" else ONE_PART))
+    for i, (k_size, v_size) in enumerate(sizes):
+        counts = [7 if i == 0 else 0] * (f["seqs"] - 1) + [page]
+        p.extend(counts)
+
+        def scaled(new, i=i):
+            new[0].mul_(k_size)
+            new[1].mul_(v_size)
+            if spoil:
+                spoil(i, new)
+        p.append(counts, seed=i, spoil=scaled)
+    rows = max(f["rows"], 3)
+    return p, [1] * (f["seqs"] - 1) + [rows], f["nq"] if form != "rows" else 2, n
+
+
+def places(counts, at):
+    """Positions: the first sequences' last tokens, then `at` over and over."""
+    return [6] * (len(counts) - 1) + [at[i % len(at)] for i in range(counts[-1])]
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_and_scales_that_keep_growing(k, act, form, hd):
+    """Each page's scores are larger than the last one's by more than the running maximum may lag, and V's scales rise and fall by powers of two: the
+    sums are scaled again and again, in registers and in tensor memory."""
+    sizes = [(0.05 * 1.45 ** i, (1.0, 0.02, 30.0, 0.5)[i % 4]) for i in range(20)]
+    p, counts, nq, n = grown(k, form, hd, sizes)
+    attend(p, form, counts, nq, gate=False)
+    attend(p, form, counts, nq, qpos=places(counts, [n - 1, 0, 200, kv8.NO_KEYS, 77, 63, 64]), seed=1)
+    p, counts, nq, n = grown(k, form, hd, sizes[::-1])
+    attend(p, form, counts, nq, seed=2)
+    attend(p, form, counts, nq, qpos=places(counts, [n - 1, 0, 200, kv8.NO_KEYS, 77, 63, 64]), seed=3)
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_poisoned_pages_reach_the_rows_that_attend_them_alone(k, act, form, hd):
+    """A K that is not finite in one head's page, a V in another's: NaN for the rows of that head that attend the page."""
+    for bad, (page_k, page_v) in ((float("nan"), (17, 18)), (float("inf"), (3, 18)), (-float("inf"), (18, 4)), (float("nan"), (0, 18))):
+        def spoil(i, new):
+            if i == page_k:
+                new[0][-3, hd + 5] = bad        # the page's last token, the second kv head
+            if i == page_v:
+                new[1][-3, 9] = bad             # the first
+        p, counts, nq, n = grown(k, form, hd, [(1.0, 1.0)] * 19, spoil=spoil)
+        assert int(np.isnan(p.model.k_scale[0, p.model.table[-1, :19]]).sum()) == 1
+        attend(p, form, counts, nq, qpos=places(counts, [n - 1, 40, 3, kv8.NO_KEYS, 16 * 17 + 2, 16 * 17 - 1, 47, 48]))
+        attend(p, form, counts, nq, qpos=places(counts, [15, 40, 3, kv8.NO_KEYS]), gate=False)
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_far_apart(k, act, form, hd):
+    """Pages of zeros, of very small and of large values side by side."""
+    top = 2.0 ** 12 if act == torch.float16 else 2.0 ** 40
+    sizes = [(1e-3, 1.0), (1.0, 1e-4), (0.0, 0.0), (0.1, 30.0), (1.0, 0.0), (0.5, 1 / top), (0.0, 1.0), (1.0, 1e-3)] * 3
+    p, counts, nq, n = grown(k, form, hd, sizes)
+    attend(p, form, counts, nq)
+    attend(p, form, counts, nq, qpos=places(counts, [n - 1, 15, 16, kv8.NO_KEYS, 31, 47, 200]), seed=1)
+    attend(p, form, counts, nq, size=0.0, seed=2)
+    p, counts, nq, n = grown(k, form, hd, [(1.0, 0.0)] * 6)      # V of zeros: zeros
+    y = attend(p, form, counts, nq)
+    assert (y[:sum(counts), :nq * hd] == 0).all()
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_queries_at_the_ends_of_their_type(k, act, form, hd):
+    small = 1e-4 if act == torch.float16 else 1.0
+    top = torch.finfo(act).max
+    p, counts, nq, n = grown(k, form, hd, [(small, 1.0)] * 6)
+    attend(p, form, counts, nq, spoil=lambda q: q.copy_(q.sign() * (top / 8 if act == torch.float16 else 1.0)))
+    attend(p, form, counts, nq, spoil=lambda q: q.mul_(torch.finfo(act).smallest_normal * 4))
+    attend(p, form, counts, nq, spoil=lambda q: q.zero_())
+    if act == torch.bfloat16:
+        attend(p, form, counts, nq, spoil=lambda q: q[:, 3:].mul_(1e-30))
+        p, counts, nq, n = grown(k, form, hd, [(2.0 ** -50, 1.0)] * 6)
+        attend(p, form, counts, nq, spoil=lambda q: q.mul_(2.0 ** 50))
+    # values that are not finite: their own row and head, and not where it attends nothing
+    start = np.concatenate([[0], np.cumsum(counts)])
+    rows, width = int(start[-1]), nq * hd
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        q = torch.ones(rows, width, dtype=act, device="cuda")
+        row = rows - 2
+        q[row, hd + 9] = bad
+        q[rows - 1, 5] = bad
+        y = torch.empty(rows, width, dtype=act, device="cuda")
+        p.ops.attention(None, p.gpu, 0, q, None, p.ints(start), p.ints(places(counts, [n - 1])[:-1] + [kv8.NO_KEYS]), y, rows, width, 0, width, nq, max(counts), 0)
+        nan = torch.isnan(y)
+        assert nan[row, hd:2 * hd].all() and int(nan.sum()) == hd and (y[rows - 1] == 0).all()
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_violations_of_a_call_skip_what_they_concern(k, act, form, hd):
+    """Positions past the end attend all there is; rows of offsets that do not hold and sequences longer than said are not written, others are."""
+    p, counts, nq, n = grown(k, form, hd, [(1.0, 1.0)] * 6)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    rows, width, first = int(start[-1]), nq * hd, int(start[-2])
+    gen = torch.Generator().manual_seed(9)
+    q = torch.randn(rows + 1, width, generator=gen).to(act).cuda()
+
+    def run(start, qpos, rows, most, max_len=0):
+        y = torch.full((len(q), width), 7.0, dtype=act, device="cuda")
+        p.ops.attention(None, p.gpu, 0, q, None, p.ints(start), None if qpos is None else p.ints(qpos), y, rows, width, 0, width, nq, most, max_len)
+        return y
+    last = places(counts, [n - 1])
+    want = run(start, last, rows, max(counts))
+    exact, tol = p.model.attention(0, q[:rows].double().cpu().numpy().reshape(rows, nq, hd), None, start, np.array(last), torch.finfo(act).eps / 2, act == torch.bfloat16)
+    k.dev.check_status()
+    got = run(start, last[:-2] + [n, 0x7FFFFFFF], rows, max(counts))
+    with pytest.raises(KernelError, match="position"):
+        k.dev.check_status()
+    assert torch.equal(got, want)
+    for s, r, most, word in ((start, rows - 1, max(counts), "offsets"), (start, rows, max(counts) - 1, "offsets"),
+                             (list(start[:-1]) + [max(int(start[-2]) - 1, 0) if len(counts) > 1 else 0xFFFFFFFF], rows, max(counts), "offsets")):
+        got = run(s, last, r, most)
+        with pytest.raises(KernelError, match=word):
+            k.dev.check_status()
+        assert (got[first:] == 7).all() and (np.abs(got[:first].double().cpu().numpy() - exact[:first]) <= tol[:first]).all()    # (another `most` may cut the rows otherwise)
+    if form != "tiles":     # max_len is what keeps the call on its form there
+        got = run(start, last, rows, max(counts), n - 1)
+        with pytest.raises(KernelError, match="max_len"):
+            k.dev.check_status()
+        assert (got[first:] == 7).all() and torch.equal(got[:first], want[:first])
+    else:
+        p.gpu.lens[-1] = p.gpu.max_pages * 16 + 1
+        got = run(start, last, rows, max(counts))
+        with pytest.raises(KernelError, match="longer"):
+            k.dev.check_status()
+        assert (got[first:] == 7).all()
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_forked_sequences_in_the_second_layer(k, act, form, hd):
+    """Two forks of one sequence grow apart and attend their own tokens behind the pages they share."""
+    p = Pair(k, layers=2, n_pages=40, nkv=2, hd=hd, n_seqs=3, max_pages=ROOM // 16 if form == "tiles" else 12, page=16)
+    nq, m = 4, {"rows": 1, "pairs": 7, "tiles": 33}[form]
+    p.extend([101, 0, 0])
+    for layer in range(2):
+        p.append([101, 0, 0], seed=5 + layer, layer=layer)
+    p.fork([0, 0], [1, 2], False)
+    p.extend([0, 1, m])
+    for layer in range(2):
+        p.append([0, 1, m], seed=7 + layer, layer=layer)
+    p.same()
+    for layer in range(2):
+        attend(p, form, [1, 1, m], nq, layer=layer, seed=layer)
+        attend(p, form, [m, m, m], nq, layer=layer, seed=3)
+    p.free([0])
+    p.compact()
+    p.same()
+    attend(p, form, [0, 1, m], nq, layer=1, seed=4)
+    k.dev.check_status()
+
+
+def test_both_parts_of_a_weight_count(k):
+    """Few rows over few keys, with small scores: the second fp16 part of the weights is what keeps fp32's accuracy."""
+    for hd, n in ((128, 5), (128, 16), (256, 9), (128, 40)):
+        p, counts, nq = filled(k, "rows", n, hd, lambda x: x * 0.2, lambda x: x)
+        p.attend(counts, nq, gate=False, size=1.0)
+        p.attend(counts, nq, gate=False, size=0.5, seed=1)
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_the_same_call_gives_the_same_bits(k, hd):
+    """Two calls that cut the keys differently, in turn and behind one another, each compared with its own first result."""
+    p, counts, nq, n = grown(k, "tiles", hd, [(0.3 * 1.2 ** i, 1.0) for i in range(40)])
+    rows, width = sum(counts), nq * hd
+    q = torch.randn(rows, width, generator=torch.Generator().manual_seed(4)).to(k.dev.act_torch).cuda()
+    start = p.ints(np.concatenate([[0], np.cumsum(counts)]))
+    y = torch.empty(rows, width, dtype=k.dev.act_torch, device="cuda")
+    first = {}
+    for i in range(120):
+        max_len = (0, n, ROOM // 2)[i % 3]
+        y.fill_(7)
+        p.ops.attention(None, p.gpu, 0, q, None, start, None, y, rows, width, 0, width, nq, max(counts), max_len)
+        if i % 4 == 0:
+            torch.cuda.synchronize()
+        assert torch.equal(y, first.setdefault(max_len, y.clone())), (i, max_len)
+    k.dev.check_status()
