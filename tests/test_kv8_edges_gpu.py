@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from decide_b200.kernels import KernelError
+from decide_b200.kernels import KernelError, Kv8Cache
 from oracle import kv8
 from tests.test_kv8_gpu import ROOM, Pair
 
@@ -442,3 +442,154 @@ def test_the_same_call_gives_the_same_bits(k, hd):
             torch.cuda.synchronize()
         assert torch.equal(y, first.setdefault(max_len, y.clone())), (i, max_len)
     k.dev.check_status()
+
+
+# ---------------------------------------------------------------- the largest and the smallest, captured calls
+
+def test_the_largest_pool(k):
+    """2^21 pages and 65,535 sequences: every page handed out, taken back, and the last of them (K and V beyond 2^32 bytes) written and attended to
+    the bit as the first ones are."""
+    n_pages, n_seqs, width, hd = 1 << 21, 65535, 32, 256
+    cache = Kv8Cache(*(torch.empty(1, n_pages, 1, 16, hd, dtype=torch.uint8, device="cuda") for _ in range(2)), *(torch.ones(1, n_pages, 1, device="cuda") for _ in range(2)),
+                     torch.zeros(n_seqs, width, dtype=torch.int32, device="cuda"), torch.zeros(n_seqs, dtype=torch.int32, device="cuda"),
+                     torch.zeros(n_pages, dtype=torch.int32, device="cuda"))
+    ops, dev = k.kv8, k.dev
+
+    def ints(x):
+        return torch.as_tensor(np.asarray(x, dtype=np.int32), device="cuda")
+    ops.extend(None, cache, ints(np.full(n_seqs, 512)))
+    dev.check_status()
+    assert torch.equal(cache.table.view(-1).long(), torch.arange(n_seqs * width, device="cuda")) and int(cache.refs.sum()) == n_seqs * width
+    ops.extend(None, cache, ints(np.eye(1, n_seqs, 3)[0]))
+    with pytest.raises(KernelError, match="longer"):
+        dev.check_status()
+    ops.fork(None, cache, ints(np.arange(0, 65534, 2)), ints(np.arange(1, 65535, 2)), 32767, True)     # copies of the even ones in the odd ones' place
+    dev.check_status()
+    assert int(cache.refs.sum()) == n_seqs * width and int(cache.refs.max()) == 1
+    ops.fork(None, cache, ints(np.arange(0, 65534, 2)), ints(np.arange(1, 65535, 2)), 32767, False)    # and shared
+    dev.check_status()
+    shared = torch.zeros(n_pages, dtype=torch.long, device="cuda").index_add_(0, cache.table.view(-1).long(), torch.ones(n_seqs * width, dtype=torch.long, device="cuda"))
+    assert torch.equal(cache.refs.long(), shared) and int(shared.max()) == 2
+    keep = [0, n_seqs - 1]
+    ops.free(None, cache, ints(np.arange(1, n_seqs - 1)), n_seqs - 2)
+    dev.check_status()
+    assert int(cache.refs.sum()) == 2 * width and cache.lens[keep].tolist() == [512, 512]
+    gen = torch.Generator().manual_seed(8)
+    new = torch.randn(2, 512, hd, generator=gen).to(dev.act_torch).cuda().repeat(1, 2, 1)
+    start = np.zeros(n_seqs + 1)
+    start[1:] = 512
+    start[-1] = 1024
+    ops.append(None, cache, 0, new[0], new[1], hd, hd, ints(start), 1024, 512)
+    for rows, nq in ((1, 4), (64, 4)):
+        start[1:], start[-1] = rows, 2 * rows
+        q = torch.randn(rows, nq * hd, generator=gen).to(dev.act_torch).cuda().repeat(2, 1)
+        y = torch.empty_like(q)
+        ops.attention(None, cache, 0, q, None, ints(start), None, y, 2 * rows, nq * hd, 0, nq * hd, nq, rows, 512)
+        dev.check_status()
+        assert torch.equal(y[:rows], y[rows:]) and torch.isfinite(y).all()
+    before = y.clone()
+    live = ints([0])
+    ops.compact(None, cache, live)
+    assert int(live) == 2 * width and int(cache.table[n_seqs - 1].max()) < 2 * width
+    ops.attention(None, cache, 0, q, None, ints(start), None, y, 2 * rows, nq * hd, 0, nq * hd, nq, rows, 512)
+    dev.check_status()
+    assert torch.equal(y, before)
+    del cache, before
+    torch.cuda.empty_cache()
+
+
+def test_the_smallest_pool(k):
+    """One page, one sequence, one token; nothing in use."""
+    p = Pair(k, n_pages=1, nkv=1, n_seqs=1, max_pages=1, page=16)
+    p.compact()
+    p.extend([0])
+    p.free([0])
+    p.attend([1], 1)                # an empty sequence: zero
+    p.extend([1])
+    p.append([1])
+    p.attend([1], 1)
+    p.attend([1], 16, qpos=[0])
+    p.extend([15])
+    p.append([15])
+    p.attend([16], 16)
+    p.compact()
+    p.same()
+    p.free([0])
+    p.compact()
+    p.same()
+    k.dev.check_status()
+
+
+def test_offsets_that_do_not_start_at_zero(k, act):
+    """Rows before the first sequence's are nobody's: not read, not written."""
+    p = Pair(k, nkv=1, n_seqs=2, page=16)
+    p.extend([20, 3])
+    gen = torch.Generator().manual_seed(1)
+    new = torch.randn(2, 30, 128, generator=gen).to(act)
+    new[:, :5] = float("nan")
+    p.ops.append(None, p.gpu, 0, new[0].cuda(), new[1].cuda(), 128, 128, p.ints([5, 25, 28]), 28, 20)
+    p.model.append(0, *(x[5:28].double().numpy().reshape(23, 1, 128) for x in new), [0, 20, 23])
+    p.same()
+    q = torch.randn(9, 128, generator=gen).to(act)
+    y = torch.full((9, 128), 7.0, dtype=act, device="cuda")
+    p.ops.attention(None, p.gpu, 0, q.cuda(), None, p.ints([4, 6, 8]), None, y, 8, 128, 0, 128, 1, 2, 20)
+    want, tol = p.model.attention(0, q[4:8].double().numpy().reshape(4, 1, 128), None, [0, 2, 4], None, torch.finfo(act).eps / 2, act == torch.bfloat16)
+    got = y.double().cpu().numpy()
+    assert (got[:4] == 7).all() and (got[8:] == 7).all() and (np.abs(got[4:8] - want) <= tol).all()
+    k.dev.check_status()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_a_captured_round_of_every_call(k, form):
+    """Fork, extend, append, attention, free and compact in one graph, replayed over restored and over changed caches: what the same calls give without
+    a graph, and the graph's rows follow the lengths of the moment."""
+    p, counts, nq, n = grown(k, form, 128, [(1.0, 1.0)] * 20)
+    seqs, page, m = len(counts), 16, counts[-1]
+    cache = Kv8Cache.empty(1, p.gpu.n_pages + 40, 2, 128, seqs + 2, p.gpu.max_pages, page)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        getattr(cache, name)[:, :p.gpu.n_pages] = getattr(p.gpu, name).view(getattr(cache, name).dtype) if name in "kv" else getattr(p.gpu, name)
+    cache.table[:seqs], cache.lens[:seqs], cache.refs[:p.gpu.n_pages] = p.gpu.table, p.gpu.lens, p.gpu.refs
+    k.kv8.extend(None, cache, p.ints([0] * (seqs + 1) + [20]))      # what is freed below
+    state = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.table, cache.lens, cache.refs)
+    saved = [t.clone() for t in state]
+    gen = torch.Generator().manual_seed(6)
+    start = p.ints([0] * (seqs + 1) + [m, m])
+    add = p.ints([0] * seqs + [m, 0])
+    new = torch.randn(2, m, 256, generator=gen).to(k.dev.act_torch).cuda()
+    q = torch.randn(m, nq * 128, generator=gen).to(k.dev.act_torch).cuda()
+    y, live = torch.zeros_like(q), p.ints([0])
+    src, dst, gone = p.ints([seqs - 1]), p.ints([seqs]), p.ints([seqs + 1])
+    max_len = 0 if form == "tiles" else 400
+    k.dev.reserve_workspace(max(k.kv8.attention_scratch_bytes(cache, nq, m, max_len), k.kv8.pages_scratch_bytes(cache)))
+
+    def round_of_calls():
+        k.kv8.fork(None, cache, src, dst, 1)
+        k.kv8.extend(None, cache, add)
+        k.kv8.append(None, cache, 0, new[0], new[1], 256, 256, start, m, m)
+        k.kv8.attention(None, cache, 0, q, None, start, None, y, m, nq * 128, 0, nq * 128, nq, m, max_len)
+        k.kv8.free(None, cache, gone, 1)
+        k.kv8.compact(None, cache, live)
+
+    def restore():
+        for t, s in zip(state, saved):
+            t.copy_(s)
+    round_of_calls()
+    k.dev.check_status()
+    want = [t.clone() for t in (*state, y, live)]
+    restore()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        round_of_calls()
+    for _ in range(3):
+        restore()
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        k.dev.check_status()
+        for a, b in zip((*state, y, live), want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))      # bits: free pages' scales are NaN
+    graph.replay()          # over what the last one left: the fork is made again
+    torch.cuda.synchronize()
+    k.dev.check_status()
+    assert torch.equal(y, want[-2]) and int(cache.lens[seqs]) == n + m
+    del graph
