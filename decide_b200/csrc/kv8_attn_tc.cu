@@ -26,7 +26,8 @@
 // shares the exponential units); the same with the tiles' exponentials in strict turns (308); scores of 128 keys in one product, which leaves
 // room for one buffer a tile (317, though the products alone take 198); fillers in a short loop of single groups (299 to 336); fillers
 // whose places are known to the compiler (543: the roles' code no longer fits the instruction cache).
-// Every wait is bounded; when one gives up the CTA raises the status word, waits for its products in flight and returns.
+// Every wait is bounded; when one gives up the CTA raises the status word, runs through its steps without waiting, stores nothing, waits for its
+// products in flight and returns.
 #include "kv8_attn.cuh"
 #include "ptx.cuh"
 
@@ -70,10 +71,22 @@ __device__ __forceinline__ void sts16(uint32_t to, uint32_t x, uint32_t y, uint3
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// A bounded wait of a whole warp: its lanes agree on whether it is over. Of lanes that saw the limit pass and lanes that saw the phase complete some
-// would leave for the CTA's barrier and the others stay at the next instruction of the whole warp, for good.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
+// A bounded wait that gives no answer: whoever called it goes on as if the phase were complete. A lane that left its loop where the others found the
+// phase complete would never meet them again at the next instruction of the whole warp; and for all lanes to agree first takes a vote, 28
+// cycles of every wait (2,048 rows over 8,191 keys: 313 us, 292 without). Once one wait has run out the others give up at once, what is worked on is
+// in bounds whatever it holds, and nothing is stored.
+__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
+    if (mbar_try_wait(bar, parity)) return;
+    const uint64_t t0 = globaltimer_ns();
+    uint32_t spins = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort_flag) return;
+        if ((++spins & 63u) == 0u && globaltimer_ns() - t0 > kWaitLimitNs) {
+            *abort_flag = 1u;
+            kv8_flag(status, code);
+            return;
+        }
+    }
 }
 
 // Advances a two-stage ring.
@@ -121,7 +134,7 @@ __device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
 // 64 keys of a warp's 32 pairs: scores out of tensor memory, their maximum, then the weights into the columns that the scores came from.
 // MASKED: some pair of the warp does not see all 64 keys; `vis` of them it does. settled(): O may be rescaled.
 template <int HD, bool MASKED, typename F>
-__device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, const float4* sc, float mul, int vis, bool scale_o, float& m, float& l, F settled) {
+__device__ __forceinline__ void softmax_half(uint32_t col_s, uint32_t col_o, const float4* sc, float mul, int vis, bool scale_o, float& m, float& l, F settled) {
     uint32_t s[2][32];
     tmem_ld_32x32(col_s, s[0]);
     tmem_ld_32x32(col_s + 32, s[1]);
@@ -149,7 +162,7 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
         l *= by;
         m = to;
         if (scale_o) {
-            if (!settled()) return false;
+            settled();
 #pragma unroll 1
             for (int c = 0; c < HD / 16; ++c) {
                 uint32_t v[16];
@@ -190,7 +203,6 @@ __device__ __forceinline__ bool softmax_half(uint32_t col_s, uint32_t col_o, con
         }
         tmem_st_32x32_x16(col_s + 16 * h, w);
     }
-    return true;
 }
 
 template <typename Act, int HD>
@@ -291,7 +303,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     const uint32_t halves = idle ? 0u : (key1 - key0 + kHalf - 1) / kHalf, steps = (halves + S::kHalves - 1) / S::kHalves;
     const uint32_t tmem = *tmem_slot;                // 0: all of it is ours
 
-    bool ok = true;                                  // this warp has not given up
     float m = kKv8None, l = 0.f;                     // softmax warps: of their pair
     if (warp > 8 || (HD == 256 && warp > 4 && warp < 8)) {
         // -------------------------------------------------------------------------------- codes -> fp16 tiles
@@ -391,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             look_up(1);
         }
         for (uint32_t i = 0; i < steps; ++i) {
-            if (i >= 2 && !(ok = warp_wait(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81))) break;
+            if (i >= 2) await(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81);
             if (w == 0 && lane < S::kGroups) {
                 const float e = kv8_log2i(v_scale);   // a NaN reaches the total through the weights, not through 1 / V scale
                 scales[(i % kScaleSlots) * 8 + lane] = make_float4(k_scale, e, isnan(e) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(e)))), 0.f);
@@ -408,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                 to_page(i + 1);
                 load(kx, 0, i + 1);
             }
-            if (i >= 2 && !(ok = warp_wait(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82))) break;
+            if (i >= 2) await(&v_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 82);
             store(vx, S::kV + ring.stage * S::kStage);
             fence_proxy_async_smem();
             __syncwarp();
@@ -436,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             const uint32_t n = halves;
             const bool both = two;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-                return warp_wait(bar, parity, abort_flag, a.status, code);
+                await(bar, parity, abort_flag, a.status, code);
+                __syncwarp();
             };
             // half u of a round of four: buffer u % 2; `last`: the stage's last product of the kind
             auto scores = [&](int x, int u, bool last) {
@@ -470,32 +482,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
                 __syncwarp();
             };
             constexpr bool kOwn = S::kHalves == 1;   // every half is a stage of its own
-            ok = wait(q_full, 0u, 83) && wait(&k_full[0], 0u, 83);
-            if (ok) {
-                tc_fence_after_sync();
-                scores(0, 0, kOwn || (!both && n == 1));
-                if (both) scores(1, 0, n == 1);
-                if (n > 1) {
-                    if (kOwn) ok = wait(&k_full[1], 0u, 83);
-                    if (kOwn) tc_fence_after_sync();
-                    if (ok) scores(0, 1, !both);
-                    if (both) scores(1, 1, true);
-                }
+            wait(q_full, 0u, 83);
+            wait(&k_full[0], 0u, 83);
+            tc_fence_after_sync();
+            scores(0, 0, kOwn || (!both && n == 1));
+            if (both) scores(1, 0, n == 1);
+            if (n > 1) {
+                if (kOwn) wait(&k_full[1], 0u, 83);
+                if (kOwn) tc_fence_after_sync();
+                scores(0, 1, !both);
+                if (both) scores(1, 1, true);
             }
             // A wait costs some 150 cycles even when it is over: each stands right behind products that were just issued.
-            for (uint32_t h0 = 0; ok && h0 < n; h0 += 4) {
+            for (uint32_t h0 = 0; h0 < n; h0 += 4) {
                 const uint32_t phase = h0 >> 2 & 1;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const uint32_t h = h0 + u;
-                    if (!ok || h >= n) break;
-                    if (!(ok = wait(&p_full[u & 1], u >> 1, 84))) break;
-                    if ((kOwn || !(u & 1)) && !(ok = wait(&v_full[u >> kShift & 1], kOwn ? u >> 1 : phase, 85))) break;
+                    if (h >= n) break;
+                    wait(&p_full[u & 1], u >> 1, 84);
+                    if (kOwn || !(u & 1)) wait(&v_full[u >> kShift & 1], kOwn ? u >> 1 : phase, 85);
                     tc_fence_after_sync();
                     const bool more = h + 2 < n, ends = kOwn || (u & 1) || h + 1 == n, next_ends = kOwn || (u & 1) || h + 3 == n;
                     values(0, u, u == 0 && h0 == 0, !both && ends, h + 1 == n);
-                    if (both && !(ok = wait(&p_full[2 + (u & 1)], u >> 1, 84))) break;
-                    if (more && (kOwn || !(u & 1)) && !(ok = wait(&k_full[(u + 2) >> kShift & 1], kOwn ? (u >> 1) ^ 1 : (u ? phase ^ 1u : phase), 86))) break;
+                    if (both) wait(&p_full[2 + (u & 1)], u >> 1, 84);
+                    if (more && (kOwn || !(u & 1))) wait(&k_full[(u + 2) >> kShift & 1], kOwn ? (u >> 1) ^ 1 : (u ? phase ^ 1u : phase), 86);
                     tc_fence_after_sync();
                     if (more) scores(0, u + 2, !both && next_ends);
                     if (both) {
@@ -541,31 +552,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
         const bool on = p < here;
         const float mul = runs && halves ? a.scale * rank[p] : 0.f;
         const uint32_t see = on ? seen[p] : most;    // pairs past the last are computed (their q is zero) and not stored
-        for (uint32_t h = 0; runs && ok && h < halves; ++h) {
+        for (uint32_t h = 0; runs && h < halves; ++h) {
             const uint32_t step = h / S::kHalves;
-            if (!(ok = warp_wait(&scale_full[step % kScaleSlots], step / kScaleSlots & 1u, abort_flag, a.status, 88))) break;
-            if (!(ok = warp_wait(&s_full[2 * x + (h & 1)], h >> 1 & 1, abort_flag, a.status, 89))) break;
+            await(&scale_full[step % kScaleSlots], step / kScaleSlots & 1u, abort_flag, a.status, 88);
+            await(&s_full[2 * x + (h & 1)], h >> 1 & 1, abort_flag, a.status, 89);
             __syncwarp();
             tc_fence_after_sync();
             const float4* sc = scales + step % kScaleSlots * 8 + 4 * (h % S::kHalves);
             const uint32_t key = key0 + h * kHalf, col_s = lanes + 128 * x + 64 * (h & 1);
             const int vis = static_cast<int>(min(see, key + kHalf)) - static_cast<int>(min(see, key));   // of the 64 keys
             auto settled = [&] {   // the V product of the last 64 keys: the one before it came before these scores, the next has no weights yet
-                const bool done = warp_wait(&pv_done[x], (h - 1) & 1u, abort_flag, a.status, 91);
+                await(&pv_done[x], (h - 1) & 1u, abort_flag, a.status, 91);
                 __syncwarp();
                 tc_fence_after_sync();
-                return done;
             };
-            if (__any_sync(0xffffffffu, vis < static_cast<int>(kHalf))) ok = softmax_half<HD, true>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
-            else ok = softmax_half<HD, false>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
-            if (!ok) break;
+            if (__any_sync(0xffffffffu, vis < static_cast<int>(kHalf))) softmax_half<HD, true>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
+            else softmax_half<HD, false>(col_s, col_o, sc, mul, vis, h > 0, m, l, settled);
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[2 * x + (h & 1)]);
         }
         // the divisor, for whoever stores the pair's columns
-        if (HD == 256 && x == 0 && ok && !idle) {
+        if (HD == 256 && x == 0 && !idle) {
             rank[p] = l == 0.f ? 0.f : whole ? 1.0f / l : 1.0f;
             __syncwarp();
             if (lane == 0) mbar_arrive(l_full);
@@ -577,13 +586,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
     // lanes of tensor memory that its number modulo four gives). A tile's q is free once its last product is done (its scores came
     // before it): rows go through 8 KB of it, 64 columns at a time, so that they leave in whole pieces. Row r keeps its 16-byte pieces at
     // piece ^ (r % 16).
-    if (warp < 8 && ok && !idle && (HD == 256 || warp < 4 || two)) {
+    if (warp < 8 && !idle && (HD == 256 || warp < 4 || two)) {
         const uint32_t x = HD == 256 ? 0 : warp >> 2, part = HD == 256 ? warp >> 2 : 0, first = HD == 256 ? 32 * (warp & 3) : 32 * warp;   // tile, 128 columns, pair of lane 0
         // (pv_done cannot tell: it may have run two phases ahead, and a wait for a phase that lies two back waits for the next one like it)
-        const bool there = (HD == 128 || warp_wait(l_full, 0u, abort_flag, a.status, 92)) && (halves == 0 || warp_wait(&o_full[x], 0u, abort_flag, a.status, 90));
-        if (there) {
-            __syncwarp();
-            tc_fence_after_sync();
+        if (HD == 256) await(l_full, 0u, abort_flag, a.status, 92);
+        if (halves) await(&o_full[x], 0u, abort_flag, a.status, 90);
+        __syncwarp();
+        tc_fence_after_sync();
+        if (__all_sync(0xffffffffu, *abort_flag == 0u)) {
             uint8_t* stage = smem + S::kQ + warp * 8192;
             const float by = HD == 256 ? rank[first + lane] : l == 0.f ? 0.f : whole ? 1.0f / l : 1.0f;   // 0: the pair attends nothing here, whatever lies in O
             const uint32_t col8 = lane & 7, col_o = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColO + 128 * (x + part);   // eight lanes a row

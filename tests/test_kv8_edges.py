@@ -13,16 +13,17 @@ def code_of(name):
     return re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
 
 
-def test_the_lanes_of_a_warp_agree_on_every_wait():
-    """The lanes of one warp that part at a wait that ran out would wait for one another without a limit. So the waits of the tcgen05 form go through
-    warp_wait, which takes a vote, but for the last one of all, whose answer nothing branches on."""
+def test_no_wait_parts_the_lanes_of_a_warp():
+    """Lanes of one warp that part at a wait that ran out would wait for one another without a limit. So the waits of the tcgen05 form give no answer that
+    anything could branch on; the one look at the flag that says whether one of them ran out is a vote of the whole warp, but for the wait loop itself and
+    the teardown behind the last barrier."""
     code = code_of("kv8_attn_tc.cu")
-    assert re.search(r"bool warp_wait\([^)]*\) \{\s*return __all_sync\(0xffffffffu, mbar_wait\([^;]*\)\);\s*\}", code)
-    calls = [m for m in re.finditer(r"(?<!\w)mbar_wait\(", code)]
-    assert len(calls) == 2
-    last = code[:calls[1].start()].rstrip()
-    assert last.endswith((";", "{", "}")), "the answer of a wait that takes no vote is used"
-    assert len(re.findall(r"warp_wait\(", code)) >= 8
+    assert re.search(r"void await\(uint64_t", code) and len(re.findall(r"(?<!\w)await\(&?\w", code)) >= 8
+    waits = [code[:m.start()].rstrip()[-1] for m in re.finditer(r"(?<!\w)mbar_wait\(", code)]
+    assert waits == [";"], "the answer of a wait is used"
+    looks = [code[:m.end()].splitlines()[-1].strip() for m in re.finditer(r"\*abort_flag\b(?! = 1u| = 0u;)", code)]
+    looks = [x for x in looks if not x.endswith("volatile uint32_t* abort_flag")]
+    assert looks == ["if (*abort_flag", "if (__all_sync(0xffffffffu, *abort_flag", "if (*abort_flag"], looks
 
 
 def test_the_tolerance_of_few_rows_sees_a_missing_second_part():
