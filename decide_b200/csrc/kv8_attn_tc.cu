@@ -18,10 +18,10 @@
 // both with one tile of 128 pairs (O has 256 columns) and stages of 64 keys; warps 5..7 then help the fillers, who have twice the codes for
 // each product (with three of them a half took 3,500 cycles).
 // Where there are fewer tiles than SMs the keys are cut into chunks, whose results a second kernel joins in chunk order.
-// Measured on the device, 32 query heads of 128 over 8 kv heads: 2,048 rows over 8,191 keys 288 us (833 TFLOP/s), 178 rows over 2,491 keys
-// 28 us; kv8_attn.cu takes 1,062 and 51. A round of both tiles' 64 keys takes about 2,000 cycles, its MMAs alone 1,250 (128x64x16 with both
-// operands in shared memory 48 each, 128x128x16 with A in tensor memory 64). What it is short of: without the softmax the same call takes
-// 241 us (one warp's issue of products; two warps 185), without its exponentials 266, without the fillers' work 259. Built and measured, and
+// Measured on the device, 32 query heads of 128 over 8 kv heads: 2,048 rows over 8,191 keys 290 us (829 TFLOP/s), 178 rows over 2,491 keys
+// 29 us; kv8_attn.cu takes 1,062 and 51. A round of both tiles' 64 keys takes about 2,000 cycles, its MMAs alone 1,250 (128x64x16 with both
+// operands in shared memory 48 each, 128x128x16 with A in tensor memory 64). What it is short of: without the softmax the same call took
+// 241 us where the whole took 288 (one warp's issue of products; two warps 185), without its exponentials 266, without the fillers' work 259. Built and measured, and
 // slower for it: a warp of products for each tile and six fillers, 512 threads (301 us: the softmax of both tiles then runs in step and
 // shares the exponential units); the same with the tiles' exponentials in strict turns (308); scores of 128 keys in one product, which leaves
 // room for one buffer a tile (317, though the products alone take 198); fillers in a short loop of single groups (299 to 336); fillers
@@ -192,7 +192,8 @@ __device__ __forceinline__ void softmax_half(uint32_t col_s, uint32_t col_o, con
                     p1 = 32 * h + 16 * g + e + 1 < vis ? p1 : 0.f;
                 }
                 // cut to fp16's 11 bits, then exact in fp16 from 2^-14 on: product and total take the same weight, and what the cut does to all
-                // of a row's weights alike cancels (of weights rounded to nearest, as kv8_attn.cu has them, the total cost three instructions each)
+                // of a row's weights alike cancels: error against 64 bits 1.2 instead of 1.3 times that of rounding the output, for 10 of 290 us of
+                // 2,048 rows over 8,191 keys (of weights rounded to nearest, as kv8_attn.cu has them, the total cost three instructions each, 57 us)
                 p0 = __uint_as_float(__float_as_uint(p0) & 0xffffe000u);
                 p1 = __uint_as_float(__float_as_uint(p1) & 0xffffe000u);
                 w[8 * g + e / 2] = ActF16::pack(p0, p1);
