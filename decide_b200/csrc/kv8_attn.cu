@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
     for (int b = 0; b < NT; ++b)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            mul[b][e] = a.scale * rank[8 * b + 2 * t + e];
+            mul[b][e] = rank[8 * b + 2 * t + e];
             m[b][e] = kKv8None;
             l[b][e] = 0.f;
         }
@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(Shape<HD, NT>::kThreads, Shape<HD, NT>::kBlock
                 }
             }
         }
-        const float ks = __shfl_sync(0xffffffffu, k_scale, i % 32), ve = kv8_log2i(__shfl_sync(0xffffffffu, v_scale, i % 32));
+        // (hd^-1/2 goes with the K scale: with q's power of two, 2^-140 for the smallest of bf16, it would leave fp32's normal numbers)
+        const float ks = a.scale * __shfl_sync(0xffffffffu, k_scale, i % 32), ve = kv8_log2i(__shfl_sync(0xffffffffu, v_scale, i % 32));
         const float back = isnan(ve) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(ve))));   // 2^-e_v; a NaN reaches the sum through the weights
         bool grow = false;
 #pragma unroll

@@ -60,7 +60,7 @@ struct Shape {
     static constexpr uint32_t kQ = 0;                    // [tiles][HD / 64]
     static constexpr uint32_t kK = kQ + kTiles * (HD / 64) * kQAtom;   // [2 stages][HD / 64]
     static constexpr uint32_t kV = kK + 2 * kStage;
-    static constexpr uint32_t kScales = kV + 2 * kStage; // float4 [kScaleSlots][8], of 16 keys: K scale, log2 of the V scale, 1 / V scale
+    static constexpr uint32_t kScales = kV + 2 * kStage; // float4 [kScaleSlots][8], of 16 keys: K scale hd^-1/2 log2(e), log2 of the V scale, 1 / V scale
     static constexpr uint32_t kRank = kScales + kScaleSlots * 8 * 16;   // float [kPairs]
     static constexpr uint32_t kSeen = kRank + kPairs * 4;   // u32 [kPairs]
     static constexpr uint32_t kBars = kSeen + kPairs * 4;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             if (i >= 2) await(&k_free[ring.stage], ring.phase ^ 1u, abort_flag, a.status, 81);
             if (w == 0 && lane < S::kGroups) {
                 const float e = kv8_log2i(v_scale);   // a NaN reaches the total through the weights, not through 1 / V scale
-                scales[(i % kScaleSlots) * 8 + lane] = make_float4(k_scale, e, isnan(e) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(e)))), 0.f);
+                scales[(i % kScaleSlots) * 8 + lane] = make_float4(a.scale * k_scale, e, isnan(e) ? 1.f : kv8_exp2i(max(-126, min(127, -static_cast<int>(e)))), 0.f);
             }
             store(kx, S::kK + ring.stage * S::kStage);
             fence_proxy_async_smem();
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_tc_kernel(const Kv8Args 
             if (lane == 0) mbar_arrive(q_full);
         }
         const bool on = p < here;
-        const float mul = runs && halves ? a.scale * rank[p] : 0.f;
+        const float mul = runs && halves ? rank[p] : 0.f;
         const uint32_t see = on ? seen[p] : most;    // pairs past the last are computed (their q is zero) and not stored
         for (uint32_t h = 0; runs && h < halves; ++h) {
             const uint32_t step = h / S::kHalves;

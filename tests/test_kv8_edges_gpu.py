@@ -593,3 +593,16 @@ def test_a_captured_round_of_every_call(k, form):
     k.dev.check_status()
     assert torch.equal(y, want[-2]) and int(cache.lens[seqs]) == n + m
     del graph
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_tiny_queries_of_huge_keys(k, act, form, hd):
+    """Queries at the small end of their type against keys at its large end, and the other way round: scores of an ordinary size."""
+    up = 2.0 ** 13 if act == torch.float16 else 2.0 ** 124
+    down = 2.0 ** -13 if act == torch.float16 else 2.0 ** -125
+    p, counts, nq, n = grown(k, form, hd, [(up, 1.0)] * 6)
+    attend(p, form, counts, nq, size=down)
+    p, counts, nq, n = grown(k, form, hd, [(2.0 ** -13 if act == torch.float16 else 2.0 ** -50, 1.0)] * 6)
+    attend(p, form, counts, nq, size=2.0 ** 13 if act == torch.float16 else 2.0 ** 50)
+    k.dev.check_status()
