@@ -606,3 +606,24 @@ def test_tiny_queries_of_huge_keys(k, act, form, hd):
     p, counts, nq, n = grown(k, form, hd, [(2.0 ** -13 if act == torch.float16 else 2.0 ** -50, 1.0)] * 6)
     attend(p, form, counts, nq, size=2.0 ** 13 if act == torch.float16 else 2.0 ** 50)
     k.dev.check_status()
+
+
+def test_part_of_a_caches_sequences(k, act):
+    """Calls over views of the table: the one sequence that brings many rows and the others that bring one each, apart."""
+    p = Pair(k, n_pages=60, nkv=2, n_seqs=4, max_pages=ROOM // 16, page=16)
+    p.extend([200, 33, 340, 1])
+    p.append([200, 33, 340, 1])
+    nq, counts = 8, [1, 1, 40, 1]
+    start = np.concatenate([[0], np.cumsum(counts)])
+    rows, width = int(start[-1]), nq * 128
+    q = torch.randn(rows, width, generator=torch.Generator().manual_seed(2)).to(act)
+    y = torch.full((rows, width), 7.0, dtype=act, device="cuda")
+    g, on = p.gpu, q.cuda()
+    many = Kv8Cache(g.k, g.v, g.k_scale, g.v_scale, g.table[2:3], g.lens[2:3], g.refs)
+    p.ops.attention(None, many, 0, on, None, p.ints(start[2:4]), None, y, rows, width, 0, width, nq, 40)
+    p.ops.attention(None, g, 0, on, None, p.ints([0, 1, 2, 2, 2]), None, y, rows, width, 0, width, nq, 1, 400)
+    last = Kv8Cache(g.k, g.v, g.k_scale, g.v_scale, g.table[3:], g.lens[3:], g.refs)
+    p.ops.attention(None, last, 0, on, None, p.ints(start[3:]), None, y, rows, width, 0, width, nq, 1, 400)
+    want, tol = p.model.attention(0, q.double().numpy().reshape(rows, nq, 128), None, start, None, torch.finfo(act).eps / 2, act == torch.bfloat16)
+    assert (np.abs(y.double().cpu().numpy() - want) <= tol).all()
+    k.dev.check_status()
